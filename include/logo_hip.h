@@ -514,6 +514,92 @@ int logo_dec_linear(const void* x, int64_t ldx, const void* w, const void* norm_
 int logo_rmsnorm(const void* x, const void* w, void* y, int64_t rows, int cols, float eps,
                  int dtype, void* stream);
 
+/*
+ * Rotary embedding by positions.  A tensor's rows: token n = b * tokens_per_batch
+ * + t and head h at x + b * x_batch + t * x_token + h * x_head (elements, the d
+ * elements of a row dense); y likewise.  y == x with equal strides: in place.
+ */
+typedef struct {
+  const void* x;
+  void* y;
+  int64_t x_batch, x_token, x_head, y_batch, y_token, y_head;
+  int32_t heads;
+} logo_rows;
+
+/*
+ * Turns the first `rot` elements (even, <= d <= 512) of each row of up to four
+ * tensors by its token's position (int32 or int64 [n_tokens], position_bits 32 or
+ * 64, of either sign): pairs (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved,
+ *   a' = amplitude (a cos t - b sin t),  b' = amplitude (b cos t + a sin t),
+ * t = position * turns[i] 2^-64 turns (turns [rot / 2] on the device, modulo one
+ * turn, so angles are exact at any position); the other elements are copied.
+ * inverse: t negated (the transpose, for the backward pass).  bf16, fp16 or fp32,
+ * computed in fp32 and rounded once, any alignment of the elements.  The
+ * counterpart of logo_rope (logo/modules/rotary.py:58-106) without cos / sin
+ * tables, for interleaved pairs, parts of a head and scaled frequencies.
+ */
+int logo_rotary(const logo_rows* rows, int n_rows, const void* positions, int position_bits, int64_t n_tokens,
+                int64_t tokens_per_batch, int d, const uint64_t* turns, int rot, int interleaved, float amplitude,
+                int inverse, int dtype, void* stream);
+
+/*
+ * A key / value cache in pages: key j of sequence b and head h is row
+ *   k + table[b * table_row + j / page_size] * k_page + h * k_head + (j % page_size) * k_slot
+ * (elements, the d elements dense; v likewise).  page_size: a power of two from 16
+ * on; strides multiples of 8, k and v 16-byte aligned.  Table entries outside [0,
+ * pages) name no page: nothing is read or written there.  cu [nseq + 1]: the
+ * tokens of a call, packed by sequence (cu[0] = 0, non-decreasing); lens [nseq]:
+ * the keys of each sequence with its new tokens included, so token i of sequence
+ * b has position lens[b] - (cu[b + 1] - cu[b]) + i.  cu, lens and table are int32
+ * device memory.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  int64_t pages;
+  const int32_t* table;
+  int64_t table_row;
+  const int32_t* cu;
+  const int32_t* lens;
+  int32_t table_width, page_size, heads, nseq;
+} logo_paged_cache;
+
+/*
+ * Append the tokens' keys and values (rows at k + n * k_token + h * k_head, v
+ * likewise; 16-bit, d = 64 or 128) to the cache, k turned by its position as
+ * logo_rotary (rot = 0: stored as it is), and turn q (may be null, with q_out)
+ * into the dense q_out [n_tokens, hq, d].  A token whose position is negative,
+ * lies behind the table or on an entry that names no page is not stored; tokens
+ * behind the last sequence (or at negative positions) are not stored and have
+ * zero rows in q_out.  The paged counterpart of logo_cache_append and
+ * logo_rope_apply (logo/cache.py:97-118, logo/layers/logo.py:132-150).
+ */
+int logo_paged_append(const logo_paged_cache* cache, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                      int64_t v_token, int64_t v_head, const void* q, int64_t q_token, int64_t q_head, void* q_out,
+                      int hq, int64_t n_tokens, int d, const uint64_t* turns, int rot, int interleaved,
+                      float amplitude, int dtype, void* stream);
+
+/* Bytes of workspace logo_paged_attn needs for the same arguments. */
+size_t logo_paged_attn_workspace_bytes(int nseq, int h, int hq, int64_t n_tokens, int d, int max_q, int max_len,
+                                       int window);
+
+/*
+ * Attention of the tokens over the cached keys of their own sequences: row (n,
+ * hq) = softmax(scale * q[n, hq] K^T) V over the keys j <= p of its kv head (and
+ * j >= p - window where window >= 0; -1: none), p the token's position.  q rows at
+ * q + n * q_token + head * q_head (multiples of 8, 16-byte aligned), out [n_tokens,
+ * hq, d] dense; 16-bit, d = 64 or 128; scale > 0.  selection (uint8 [n_tokens], may
+ * be null): a token whose entry is zero reads no key and gets zero rows (LoGo's
+ * gate, logo/layers/logo.py:186-209, :228-249).  Rows that see no key are zero.
+ * Rows behind the last sequence are zero with zero_rest, else left as they are.
+ * max_q, max_len: bounds on the new tokens and on the keys of a sequence, which
+ * size the launch; larger ones on the device stay right but slow.
+ */
+int logo_paged_attn(const logo_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head, void* out,
+                    const uint8_t* selection, int hq, int64_t n_tokens, int d, int max_q, int max_len, float scale,
+                    int window, int zero_rest, void* workspace, size_t workspace_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

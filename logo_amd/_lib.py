@@ -5,6 +5,7 @@ PyTorch fallback: if the library is missing, or a tensor is not on a ROCm GPU,
 the ops raise.
 """
 
+import contextlib
 import ctypes
 import os
 import re
@@ -69,6 +70,29 @@ SIGNATURES = {
                          _I, _P],
                         _I),
 }
+# The structs of include/logo_hip.h, passed by address.
+class Rows(ctypes.Structure):
+    """``logo_rows``."""
+
+    _fields_ = [("x", _P), ("y", _P)] + [(n, _I64) for n in ("x_batch", "x_token", "x_head", "y_batch", "y_token",
+                                                             "y_head")] + [("heads", ctypes.c_int32)]
+
+
+class PagedCacheArg(ctypes.Structure):
+    """``logo_paged_cache``."""
+
+    _fields_ = ([("k", _P), ("v", _P)] + [(n, _I64) for n in ("k_page", "k_head", "k_slot", "v_page", "v_head", "v_slot",
+                                                              "pages")]
+                + [("table", _P), ("table_row", _I64), ("cu", _P), ("lens", _P)]
+                + [(n, ctypes.c_int32) for n in ("table_width", "page_size", "heads", "nseq")])
+
+
+SIGNATURES["logo_rotary"] = ([ctypes.POINTER(Rows), _I, _P, _I, _I64, _I64, _I, _P, _I, _I, _F, _I, _I, _P], _I)
+SIGNATURES["logo_paged_append"] = ([ctypes.POINTER(PagedCacheArg)] + [_P, _I64, _I64] * 3
+                                   + [_P, _I, _I64, _I, _P, _I, _I, _F, _I, _P], _I)
+SIGNATURES["logo_paged_attn_workspace_bytes"] = ([_I, _I, _I, _I64, _I, _I, _I, _I], _SZ)
+SIGNATURES["logo_paged_attn"] = ([ctypes.POINTER(PagedCacheArg), _P, _I64, _I64, _P, _P, _I, _I64, _I, _I, _I, _F, _I, _I,
+                                  _P, _SZ, _I, _P], _I)
 _BWD = ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P,
          _SZ, _P], _I)
 for _name in ("logo_sq_bwd", "logo_sq_bwd_delta", "logo_sq_bwd_dq", "logo_sq_bwd_dkv", "logo_sq_bwd_dqkv"):
@@ -139,6 +163,14 @@ def ptr(t):
 def stream_of(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (a launch goes to the
+    current device, whatever device its stream belongs to)."""
+    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
 
 # Optional per-launch timing hook: called as hook(name, "start"|"end") around
 # every kernel launch of the ops (bench.py records HIP events through it).

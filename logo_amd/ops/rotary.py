@@ -1,0 +1,197 @@
+"""Rotary embedding by positions (``csrc/rotary.hip``).
+
+``rotary`` is differentiable and returns new tensors, ``rotary_`` rotates in
+place.  Where ``ops.glue.rope`` takes bf16 cos / sin tables of whole heads and
+rounds every product as the eager chain of logo/modules/rotary.py:81-106 does,
+these take token positions and a ``RotaryPlan``: half or interleaved pairs, the
+first part of a head or all of it, frequencies scaled for contexts longer than
+the trained ones, bf16, fp16 and fp32, any strides; angles are exact at any
+position, products are in fp32 and rounded once.
+"""
+
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .. import _lib
+
+__all__ = ["RotaryPlan", "rotary_plan", "rotary", "rotary_", "RotaryFunction"]
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+MAX_HEAD_DIM = 512
+
+
+@dataclass(frozen=True)
+class RotaryPlan:
+    """How heads are rotated (``rotary_plan`` makes one): the first ``rot_dim``
+    of ``head_dim`` elements, in pairs ``(i, i + rot_dim / 2)`` or, with
+    ``interleaved``, ``(2 i, 2 i + 1)``; pair i turns by ``turns[i]`` 2^-64 turns
+    per position (int64 ``[rot_dim / 2]`` on the device, the bits of an unsigned
+    value) and is multiplied by ``amplitude``."""
+
+    head_dim: int
+    rot_dim: int
+    interleaved: bool
+    amplitude: float
+    turns: torch.Tensor
+
+    def to(self, device) -> "RotaryPlan":
+        return RotaryPlan(self.head_dim, self.rot_dim, self.interleaved, self.amplitude, self.turns.to(device))
+
+
+def rotary_plan(head_dim: int, theta: float = 10000.0, rot_dim: Optional[int] = None, interleaved: bool = False,
+                scaling: Optional[str] = None, factor: float = 1.0, trained_len: Optional[int] = None,
+                device=None) -> RotaryPlan:
+    """The plan of frequencies ``f_i = theta^(-2 i / rot_dim)`` radians per
+    position (logo/modules/rotary.py:58-78), scaled for a context ``factor``
+    times the trained one:
+
+    * ``"linear"``: positions interpolated, ``f_i / factor``;
+    * ``"ntk"``: the base stretched, ``theta * factor^(rot_dim / (rot_dim - 2))``:
+      the fastest pair keeps its frequency, the slowest is divided by ``factor``
+      (a single pair keeps its own);
+    * ``"yarn"``: pairs that turn more than 32 times over ``trained_len``
+      positions keep their frequency, those that turn less than once are divided
+      by ``factor``, linearly in the number of turns between; cos and sin are
+      multiplied by ``0.1 ln(factor) + 1``."""
+    rot = head_dim if rot_dim is None else int(rot_dim)
+    if not 1 <= head_dim <= MAX_HEAD_DIM:
+        raise ValueError(f"head_dim must be in [1, {MAX_HEAD_DIM}], got {head_dim}")
+    if rot < 0 or rot > head_dim or rot % 2:
+        raise ValueError(f"rot_dim must be even and at most head_dim ({head_dim}), got {rot}")
+    if not (theta > 0 and math.isfinite(theta)):
+        raise ValueError(f"theta must be positive, got {theta}")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    if not (factor > 0 and math.isfinite(factor)):
+        raise ValueError(f"factor must be positive, got {factor}")
+    if scaling == "yarn" and (factor < 1 or not trained_len or trained_len < 1):
+        raise ValueError("scaling 'yarn' needs trained_len and a factor of at least 1")
+    if scaling == "ntk" and rot > 2:
+        theta = theta * factor ** (rot / (rot - 2))
+    freqs = [theta ** (-i / rot) for i in range(0, rot, 2)]
+    amplitude = 1.0
+    if scaling == "linear":
+        freqs = [f / factor for f in freqs]
+    elif scaling == "yarn":
+        keep = [min(max((trained_len * f / (2 * math.pi) - 1.0) / 31.0, 0.0), 1.0) for f in freqs]
+        freqs = [f * k + f / factor * (1.0 - k) for f, k in zip(freqs, keep)]
+        amplitude = 0.1 * math.log(factor) + 1.0
+    # turns modulo one in 64-bit fixed point, as the bits of an int64
+    turns = [int(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for f in freqs]
+    turns = [t - (1 << 64) if t >> 63 else t for t in turns]
+    return RotaryPlan(int(head_dim), rot, bool(interleaved), amplitude,
+                      torch.tensor(turns, dtype=torch.int64).to(device=device))
+
+
+def batch_token_strides(x: torch.Tensor):
+    """(batch, token, head) strides of ``[T, H, D]`` or ``[B, T, H, D]`` rows, 0
+    where a size of one makes a stride meaningless."""
+    s = [st if n > 1 else 0 for st, n in zip(x.stride()[:-1], x.shape[:-1])]
+    return (0, *s) if len(s) == 2 else tuple(s)
+
+
+def _check(xs, positions, plan, what):
+    if not 1 <= len(xs) <= 4:
+        raise ValueError(f"{what} takes one to four tensors")
+    x0 = xs[0]
+    for x in xs:
+        if x.dim() < 3 or x.shape[:-2] != x0.shape[:-2] or x.shape[-1] != plan.head_dim or x.dtype != x0.dtype:
+            raise ValueError(f"{what} needs [..., T, H, D] tensors of one type and shape prefix, D = {plan.head_dim}")
+    if x0.dtype not in _DTYPES:
+        raise ValueError(f"{what} takes bf16, fp16 or fp32 tensors, got {x0.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: positions must be int32 or int64")
+    lead = x0.shape[:-2]
+    if positions.dim() > len(lead) or any(p != n and p != 1 for p, n in zip(positions.shape[::-1], lead[::-1])):
+        raise ValueError(f"{what}: positions {tuple(positions.shape)} do not match the tokens {tuple(lead)}")
+    _lib.require_gpu(*xs, positions, plan.turns)
+    if any(t.device != x0.device for t in (*xs, positions, plan.turns)):
+        raise ValueError(f"{what}: tensors on different devices")
+
+
+def _launch(xs, ys, positions, plan, inverse):
+    """``ys`` <- rotated ``xs``, all ``[T, H, D]`` or ``[B, T, H, D]`` with dense rows."""
+    x0 = xs[0]
+    lead = x0.shape[:-2]
+    pos = positions.expand(lead).contiguous()
+    rows = (_lib.Rows * len(xs))()
+    live = 0
+    for x, y in zip(xs, ys):
+        if x.numel() == 0:
+            continue
+        r = rows[live]
+        r.x, r.y, r.heads = x.data_ptr(), y.data_ptr(), x.shape[-2]
+        r.x_batch, r.x_token, r.x_head = batch_token_strides(x)
+        r.y_batch, r.y_token, r.y_head = batch_token_strides(y)
+        live += 1
+    if live == 0:
+        return
+    with _lib.on_device(x0):
+        _lib.launch("logo_rotary", _lib.lib().logo_rotary, rows, live, _lib.ptr(pos), 32 if pos.dtype == torch.int32
+                    else 64, pos.numel(), lead[-1], plan.head_dim, _lib.ptr(plan.turns), plan.rot_dim,
+                    int(plan.interleaved), plan.amplitude, int(inverse), _DTYPES[x0.dtype], _lib.stream_of(x0))
+
+
+def _rows4(x):
+    """``x [..., T, H, D]`` with dense rows and at most one batch axis (a copy where it has none)."""
+    if x.dim() > 4:
+        x = x.reshape(-1, *x.shape[-3:])
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+class RotaryFunction(torch.autograd.Function):
+    """``rotary`` as one autograd node: one launch forward, one (the transposed
+    rotation of the gradients that arrive) backward."""
+
+    @staticmethod
+    def forward(ctx, positions, plan, inverse, *xs):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.plan, ctx.inverse = plan, inverse
+        ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+        pos = positions
+        if xs[0].dim() > 4:
+            pos = positions.expand(xs[0].shape[:-2]).reshape(-1, xs[0].shape[-3])
+        _launch([_rows4(x) for x in xs], [_rows4(y) for y in ys], pos, plan, inverse)
+        return tuple(ys)
+
+    @staticmethod
+    def backward(ctx, *gys):
+        positions, = ctx.saved_tensors
+        live = [i for i, g in enumerate(gys) if g is not None]
+        gxs = [None] * len(gys)
+        if live:
+            for i, g in zip(live, RotaryFunction.apply(positions, ctx.plan, not ctx.inverse, *(gys[i] for i in live))):
+                gxs[i] = g
+        return (None, None, None, *gxs)
+
+
+def rotary(tensors, positions, plan: RotaryPlan):
+    """Rotate ``[..., T, H_i, D]`` tensors (one to four of one shape prefix) by
+    their tokens' ``positions`` (int32 or int64, broadcast to ``[..., T]``, of
+    either sign); returns new contiguous tensors.  Differentiable."""
+    xs = list(tensors)
+    _check(xs, positions, plan, "rotary")
+    return list(RotaryFunction.apply(positions, plan, False, *xs))
+
+
+def rotary_(tensors, positions, plan: RotaryPlan):
+    """``rotary`` in place, without gradients; returns the tensors.  At most one
+    batch axis, dense rows, and no two rows in the same memory."""
+    xs = list(tensors)
+    _check(xs, positions, plan, "rotary_")
+    for x in xs:
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise ValueError("rotary_ has no gradient; use rotary")
+        if x.dim() > 4 or (x.stride(-1) != 1 and x.shape[-1] > 1):
+            raise ValueError("rotary_ needs [T, H, D] or [B, T, H, D] tensors with dense rows")
+        extent = x.shape[-1]
+        for st, n in sorted((st, n) for st, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
+            if st < extent:
+                raise ValueError("rotary_: rows share memory")
+            extent = st * (n - 1) + extent
+    _launch(xs, xs, positions, plan, False)
+    return xs

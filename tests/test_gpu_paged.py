@@ -1,0 +1,305 @@
+"""GPU parity of the paged append and the paged attention against 64-bit
+arithmetic, on pools whose unused slots and pages hold NaN."""
+
+import math
+
+import pytest
+import torch
+
+from logo_amd.ops.paged import paged_append, paged_attn
+from logo_amd.ops.rotary import rotary_plan
+from tests import paged_ref as ref
+from tests.helpers import gen
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def _dev(ts, gpu):
+    """The tensors on the device with their strides."""
+    out = []
+    for t in ts:
+        d = torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=gpu)
+        out.append(d.copy_(t))
+    return out
+
+
+def _run(gpu, new, lens, HQ, H, D, page, dtype, seed, tail=0, select=None, order="page", **kw):
+    g = gen(seed)
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, H, D, page, dtype, g, order=order)
+    N = sum(new) + tail
+    q = torch.randn(N, HQ, D, generator=g).to(dtype)
+    sel = None
+    if select is not None:
+        sel = torch.rand(N, generator=g) < select
+    r, mag = ref.paged_attn(q, kp, vp, table, cu, ln, selection=sel, **kw)
+    args = [t.to(gpu) for t in (kp, vp, table, cu, ln)]
+    o = paged_attn(q.to(gpu), *args, selection=None if sel is None else sel.to(gpu), max_q=max(new + [0]),
+                   max_len=max(lens + [0]), **kw)
+    ref.check("o", o, r, ref.attn_bound(r, mag, dtype))
+    # bounds left to their defaults may cut the keys otherwise, within the same bound
+    o2 = paged_attn(q.to(gpu), *args, selection=None if sel is None else sel.to(gpu), **kw)
+    ref.check("o, default bounds", o2, r, ref.attn_bound(r, mag, dtype))
+    return o
+
+
+# lengths around tiles, pages and pieces; no keys before the chunk; a sequence without new tokens; one without keys
+RAGGED = ([1, 0, 5, 33, 1, 64, 2], [1, 40, 5, 100, 700, 64, 1029])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("HQ,H,D,page", [(4, 4, 128, 16), (6, 2, 64, 32), (8, 1, 128, 64), (5, 1, 64, 16), (2, 2, 64, 1024)])
+@pytest.mark.parametrize("kw", [dict(), dict(window=0), dict(window=37, select=0.5), dict(select=0.3, tail=7, scale=0.2)],
+                         ids=lambda k: "-".join(k) or "plain")
+def test_ragged(gpu, dtype, HQ, H, D, page, kw):
+    _run(gpu, *RAGGED, HQ, H, D, page, dtype, seed=HQ + D, **kw)
+
+
+@pytest.mark.parametrize("HQ,H,D", [(4, 4, 128), (8, 2, 64), (64, 1, 128), (40, 2, 128)])
+@pytest.mark.parametrize("lens", [[1], [300, 31, 1000, 2], [5000, 4097]])
+def test_single_tokens(gpu, HQ, H, D, lens):
+    """A decode step: the keys of long rows are cut into pieces and joined."""
+    _run(gpu, [1] * len(lens), lens, HQ, H, D, 16, BF16, seed=sum(lens))
+    _run(gpu, [1] * len(lens), lens, HQ, H, D, 64, F16, seed=sum(lens) + 1, select=0.5, window=200)
+
+
+@pytest.mark.parametrize("new,lens", [([130], [130]), ([257], [1300]), ([200, 1, 129], [900, 2000, 129]), ([513], [700])])
+@pytest.mark.parametrize("kw", [dict(), dict(window=128), dict(select=0.25), dict(select=0.25, window=100)],
+                         ids=lambda k: "-".join(k) or "plain")
+@pytest.mark.parametrize("HQ,H,D", [(2, 2, 128), (4, 1, 64)])
+def test_chunks(gpu, new, lens, kw, HQ, H, D):
+    _run(gpu, new, lens, HQ, H, D, 16, BF16, seed=sum(new), **kw)
+
+
+@pytest.mark.parametrize("order", ["page", "slot", "pair"])
+def test_pool_and_query_strides(gpu, order):
+    new, lens = RAGGED
+    g = gen(11)
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 2, 64, 16, BF16, g, order=order)
+    N = sum(new)
+    rows = torch.randn(N, 3 * 4 * 64 + 8, generator=g).bfloat16()
+    q = rows[:, 4 * 64:8 * 64].unflatten(1, (4, 64))
+    r, mag = ref.paged_attn(q, kp, vp, table, cu, ln)
+    rg = rows.to(gpu)
+    qg = rg[:, 4 * 64:8 * 64].unflatten(1, (4, 64))
+    wide = torch.full((table.shape[0], 2 * table.shape[1]), 7, dtype=torch.int32, device=gpu)
+    wide[:, ::2] = table.to(gpu)
+    for tb in (table.to(gpu), wide[:, ::2]):
+        if order == "pair":
+            both = torch.stack([kp, vp], dim=1).to(gpu)
+            pools = [both[:, 0], both[:, 1]]
+        else:
+            pools = _dev([kp, vp], gpu)
+        o = paged_attn(qg, *pools, tb, cu.to(gpu), ln.to(gpu), max_q=64, max_len=1029)
+        ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
+    # heads before tokens, and rows at odd addresses
+    qt = q.transpose(0, 1).contiguous().to(gpu).transpose(0, 1)
+    odd = torch.empty(N * 4 * 64 + 1, dtype=BF16, device=gpu)[1:].view(N, 4, 64).copy_(q)
+    for x in (qt, odd):
+        o = paged_attn(x, *[t.to(gpu) for t in (kp, vp, table, cu, ln)], max_q=64, max_len=1029)
+        ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
+
+
+def test_rows_of_no_sequence_and_of_no_key(gpu):
+    """Rows behind the last sequence: zero, or left alone in a caller's out; tokens at negative positions see nothing;
+    an unselected call reads nothing."""
+    g = gen(12)
+    new, lens = [4, 3, 40], [2, 0, 300]
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 2, 64, 16, BF16, g)
+    N = sum(new) + 9
+    q = torch.randn(N, 4, 64, generator=g).bfloat16()
+    r, mag = ref.paged_attn(q, kp, vp, table, cu, ln)
+    args = [t.to(gpu) for t in (kp, vp, table, cu, ln)]
+    for bounds in (dict(max_q=40, max_len=300), dict(max_q=1, max_len=1), dict(max_q=40, max_len=4000), dict()):
+        out = torch.full((N, 4, 64), 7.0, dtype=BF16, device=gpu)
+        got = paged_attn(q.to(gpu), *args, out=out, **bounds)
+        assert got is out and bool((out[sum(new):] == 7).all())
+        ref.check("o", out[:sum(new)], r[:sum(new)], ref.attn_bound(r, mag, BF16)[:sum(new)])
+        o = paged_attn(q.to(gpu), *args, **bounds)
+        assert bool((o[sum(new):] == 0).all()) and bool((o[:2] == 0).all()) and bool((o[4:7] == 0).all())
+        o = paged_attn(q.to(gpu), *args, selection=torch.zeros(N, dtype=torch.bool, device=gpu), **bounds)
+        assert bool((o == 0).all())
+    empty = torch.zeros(0, dtype=torch.int32, device=gpu)
+    o = paged_attn(q.to(gpu), args[0], args[1], empty.view(0, 3), torch.zeros(1, dtype=torch.int32, device=gpu), empty)
+    assert bool((o == 0).all())
+
+
+def test_entries_that_name_no_page(gpu):
+    """Keys of pages that the table does not name (freed behind a window, or out of range) are not seen."""
+    g = gen(13)
+    new, lens = [1, 20, 150], [500, 400, 600]
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 2, 128, 16, BF16, g)
+    table[0, :20] = -1
+    table[1, 3] = kp.shape[0]
+    table[1, 7] = -2147483648
+    table[2, 30:36] = 2147483647
+    table[2, 0] = -5
+    q = torch.randn(sum(new), 4, 128, generator=g).bfloat16()
+    args = [t.to(gpu) for t in (kp, vp, table, cu, ln)]
+    for kw in (dict(), dict(window=100)):
+        r, mag = ref.paged_attn(q, kp, vp, table, cu, ln, **kw)
+        for bounds in (dict(max_q=150, max_len=600), dict()):
+            o = paged_attn(q.to(gpu), *args, **kw, **bounds)
+            ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
+
+
+def test_large_scores_and_infinities(gpu):
+    """Scores of thousands stay finite; a key of infinities or NaN spoils only the rows that see it."""
+    g = gen(14)
+    new, lens = [70], [200]
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 1, 64, 16, BF16, g)
+    q = torch.randn(70, 2, 64, generator=g).bfloat16() * 40
+    r, mag = ref.paged_attn(q, kp * 8, vp, table, cu, ln)
+    args = [t.to(gpu) for t in (table, cu, ln)]
+    o = paged_attn(q.to(gpu), (kp * 8).to(gpu), vp.to(gpu), *args)
+    # |q| |k| scale is 320 times the bound's: 0.064 of sum p |v|, where two scores lie within it of each other
+    ref.check("o", o, r, ref.half_step(BF16) * (mag + r.abs()) + 0.064 * mag)
+    # query rows of NaN, keys and values of NaN and infinity at the chunk's last token
+    r, mag = ref.paged_attn(q / 40, kp, vp, table, cu, ln)
+    last = table[0, 199 // 16].item()
+    for bad in (math.nan, math.inf, -math.inf):
+        k2, v2, q2 = kp.clone(), vp.clone(), q / 40
+        k2[last, 0, 199 % 16] = bad
+        v2[last, 0, 199 % 16] = bad
+        q2[3] = math.nan
+        for bounds in (dict(max_q=70, max_len=200), dict(max_len=100000)):
+            o = paged_attn(q2.to(gpu), k2.to(gpu), v2.to(gpu), *args, **bounds).cpu()
+            keep = [i for i in range(69) if i != 3]
+            ref.check("o", o[keep], r[keep], ref.attn_bound(r, mag, BF16)[keep])
+            assert bool(o[3].isnan().all())
+            assert not bool(o[69].isfinite().any())
+
+
+def test_streams_and_replays(gpu):
+    """A decode step captured into two graphs that replay in turn, lengths growing on the device between replays."""
+    g = gen(15)
+    new, lens = [1, 1, 1], [900, 30, 1500]
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 2, 128, 16, BF16, g)
+    q = torch.randn(3, 8, 128, generator=g).bfloat16().to(gpu)
+    args = [t.to(gpu) for t in (kp, vp, table, cu, ln)]
+    side = torch.cuda.Stream(device=gpu)
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        paged_attn(q, *args, max_q=1, max_len=1600)
+        for w in (None, 64):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                outs.append(paged_attn(q, *args, max_q=1, max_len=1600, window=w))
+            graphs.append(graph)
+    torch.cuda.current_stream().wait_stream(side)
+    for step in range(4):
+        for graph, out, w in zip(graphs, outs, (None, 64)):
+            graph.replay()
+            eager = paged_attn(q, *args, max_q=1, max_len=1600, window=w)
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager) and bool(out.isfinite().all())
+            r, mag = ref.paged_attn(q.cpu(), kp, vp, table, cu, ln - step, window=w)
+            ref.check("o", out, r, ref.attn_bound(r, mag, BF16))
+        args[4].sub_(1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("order", ["page", "slot", "pair"])
+@pytest.mark.parametrize("kw", [None, dict(), dict(rot_dim=32, interleaved=True, scaling="ntk", factor=4.0)],
+                         ids=["none", "plain", "part"])
+def test_append(gpu, dtype, order, kw):
+    """Every new key and value in its slot, every other slot as it was, q rotated; stacked [q | k | v] rows."""
+    D, H, HQ = 64, 2, 4
+    g = gen(16)
+    new, lens = [1, 0, 5, 33, 1, 64, 2, 4], [1, 40, 5, 100, 700, 64, 1029, 2]
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, H, D, 16, dtype, g, order=order)
+    table[6, 1028 // 16] = -1     # the last token's page is not held
+    tail = 3
+    N = sum(new) + tail
+    rows = torch.randn(N, (HQ + 2 * H) * D, generator=g).to(dtype)
+    q, k, v = (t.unflatten(1, (-1, D)) for t in rows.split((HQ * D, H * D, H * D), dim=1))
+    pos = torch.cat([torch.arange(t - n, t) for n, t in zip(new, lens)] + [torch.zeros(tail, dtype=torch.int64)])
+    rot = kw.get("rot_dim", D) if kw is not None else 0
+    f, amp = ref.frequencies(rot, **{a: b for a, b in (kw or {}).items() if a in ("scaling", "factor")})
+    inter = bool(kw and kw.get("interleaved"))
+    rk, mk = ref.rotate(k, pos, rot, inter, f, amp)
+    rq, mq = ref.rotate(q, pos, rot, inter, f, amp)
+    if order == "pair":
+        both = torch.stack([kp, vp], dim=1).to(gpu)
+        kg, vg = both[:, 0], both[:, 1]
+    else:
+        kg, vg = _dev([kp, vp], gpu)
+    plan = rotary_plan(D, device=gpu, **kw) if kw is not None else None
+    rg = rows.to(gpu)
+    qg, kn, vn = (t.unflatten(1, (-1, D)) for t in rg.split((HQ * D, H * D, H * D), dim=1))
+    qo = paged_append(kn, vn, kg, vg, table.to(gpu), cu.to(gpu), ln.to(gpu), q=qg, plan=plan)
+    gone = (pos < 0) | (torch.arange(N) >= sum(new))
+    rq[gone], mq[gone] = 0, 0
+    ref.check("q", qo, rq, ref.rotate_bound(rq, mq, dtype))
+    kc, vc = kg.cpu(), vg.cpu()
+    at = 0
+    for s, n in enumerate(new):
+        for i in range(n):
+            p, t = lens[s] - n + i, at + i
+            page = int(table[s, p // 16]) if p >= 0 else -1
+            if page < 0:
+                continue
+            ref.check("k", kc[page, :, p % 16], rk[t], ref.rotate_bound(rk[t], mk[t], dtype))
+            assert torch.equal(vc[page, :, p % 16], v[t])
+            kc[page, :, p % 16], vc[page, :, p % 16] = kp[page, :, p % 16], vp[page, :, p % 16]
+        at += n
+    assert torch.equal(kc.view(torch.int16), kp.contiguous().view(torch.int16))
+    assert torch.equal(vc.view(torch.int16), vp.contiguous().view(torch.int16))
+
+
+def test_append_many_sequences_and_no_tokens(gpu):
+    """More sequences than a wave has lanes, most of them without new tokens."""
+    g = gen(17)
+    new = [1 if i % 3 == 0 else 0 for i in range(200)]
+    lens = [i % 50 + 1 for i in range(200)]
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 1, 128, 16, BF16, g)
+    N = sum(new)
+    k, v = (torch.randn(N, 1, 128, generator=g).bfloat16() for _ in range(2))
+    args = [t.to(gpu) for t in (kp, vp, table, cu, ln)]
+    assert paged_append(k.to(gpu), v.to(gpu), *args) is None
+    t = 0
+    for s, n in enumerate(new):
+        if n:
+            p = lens[s] - 1
+            assert torch.equal(args[0][int(table[s, p // 16]), 0, p % 16].cpu(), k[t, 0])
+            assert torch.equal(args[1][int(table[s, p // 16]), 0, p % 16].cpu(), v[t, 0])
+            t += 1
+    assert paged_append(k[:0].to(gpu), v[:0].to(gpu), *args) is None
+
+
+def test_append_then_attend(gpu):
+    """Prompts in chunks, then single tokens, as a server runs them: the same outputs as whole sequences in 64 bits."""
+    g = gen(18)
+    D, H, HQ, page = 64, 2, 4, 32
+    total = [150, 70]
+    plan = rotary_plan(D, device=gpu)
+    f, _ = ref.frequencies(D)
+    q, k, v = ([torch.randn(t, h, D, generator=g).bfloat16() for t in total] for h in (HQ, H, H))
+    kp, vp = (torch.full((12, H, page, D), math.nan, dtype=BF16, device=gpu) for _ in range(2))
+    table = torch.tensor([[3, 0, 11, 5, 7], [1, 9, 2, -1, -1]], dtype=torch.int32, device=gpu)
+    done = [0, 0]
+    outs = [[], []]
+    for new in ([64, 0], [60, 33], [1, 36], [24, 1], [1, 0]):
+        cu = torch.tensor([0, new[0], new[0] + new[1]], dtype=torch.int32, device=gpu)
+        cut = lambda x: torch.cat([x[s][done[s]:done[s] + new[s]] for s in range(2)]).to(gpu)  # noqa: E731
+        done_after = [d + n for d, n in zip(done, new)]
+        lens = torch.tensor(done_after, dtype=torch.int32, device=gpu)
+        qr = paged_append(cut(k), cut(v), kp, vp, table, cu, lens, q=cut(q), plan=plan)
+        o = paged_attn(qr, kp, vp, table, cu, lens, max_q=max(new), max_len=max(done_after)).cpu()
+        outs[0].append(o[:new[0]])
+        outs[1].append(o[new[0]:])
+        done = done_after
+    assert done == total
+    for s in range(2):
+        t = total[s]
+        pos = torch.arange(t)
+        rot = lambda x: ref.rotate(x, pos, D, False, f)[0].to(BF16)  # noqa: E731  rounded where the kernel rounds
+        pools = [torch.zeros(1, H, 256, D, dtype=BF16) for _ in range(2)]
+        pools[0][0, :, :t], pools[1][0, :, :t] = rot(k[s]).transpose(0, 1), v[s].transpose(0, 1)
+        r, mag = ref.paged_attn(rot(q[s]), *pools, torch.zeros(1, 1, dtype=torch.int32),
+                                torch.tensor([0, t]), torch.tensor([t]))
+        # a rotated value that fp32 puts on the other side of a rounding border is off by a whole step: at most a few,
+        # each moving a score by 2^-7 of one of 64 products
+        ref.check("o", torch.cat(outs[s]), r, ref.attn_bound(r, mag, BF16) + 2.0 ** -8 * mag)
