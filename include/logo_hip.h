@@ -580,9 +580,9 @@ int logo_paged_append(const logo_paged_cache* cache, const void* k, int64_t k_to
                       int hq, int64_t n_tokens, int d, const uint64_t* turns, int rot, int interleaved,
                       float amplitude, int dtype, void* stream);
 
-/* Bytes of workspace logo_paged_attn needs for the same arguments. */
+/* Bytes of workspace logo_paged_attn needs for the same arguments (selected: with a selection). */
 size_t logo_paged_attn_workspace_bytes(int nseq, int h, int hq, int64_t n_tokens, int d, int max_q, int max_len,
-                                       int window);
+                                       int window, int selected);
 
 /*
  * Attention of the tokens over the cached keys of their own sequences: row (n,

@@ -90,7 +90,7 @@ class PagedCacheArg(ctypes.Structure):
 SIGNATURES["logo_rotary"] = ([ctypes.POINTER(Rows), _I, _P, _I, _I64, _I64, _I, _P, _I, _I, _F, _I, _I, _P], _I)
 SIGNATURES["logo_paged_append"] = ([ctypes.POINTER(PagedCacheArg)] + [_P, _I64, _I64] * 3
                                    + [_P, _I, _I64, _I, _P, _I, _I, _F, _I, _P], _I)
-SIGNATURES["logo_paged_attn_workspace_bytes"] = ([_I, _I, _I, _I64, _I, _I, _I, _I], _SZ)
+SIGNATURES["logo_paged_attn_workspace_bytes"] = ([_I, _I, _I, _I64, _I, _I, _I, _I, _I], _SZ)
 SIGNATURES["logo_paged_attn"] = ([ctypes.POINTER(PagedCacheArg), _P, _I64, _I64, _P, _P, _I, _I64, _I, _I, _I, _F, _I, _I,
                                   _P, _SZ, _I, _P], _I)
 _BWD = ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P,

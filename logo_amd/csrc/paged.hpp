@@ -1,7 +1,10 @@
 // The paged key / value cache as the kernels that write and read it see it.
 #pragma once
 
+#include <math.h>
+
 #include "capi.hpp"
+#include "common.hpp"
 
 namespace logo {
 
@@ -26,5 +29,157 @@ inline int paged_check(const logo_paged_cache* c, int d) {
   LOGO_REQUIRE(c->nseq == 0 || (c->cu && c->lens && (c->table || c->table_width == 0)), "null table, cu or lens");
   return LOGO_OK;
 }
+
+struct PagedArgs {
+  logo_paged_cache c;
+  const bf16* q;
+  int64_t q_token, q_head;
+  bf16* out;             // [n, hq, D]
+  const uint8_t* sel;    // [n] or null: every token
+  int32_t* idx;          // [n] with sel: the selected tokens of each sequence, from its first token's place on
+  int32_t* count;        // [nseq] with sel: how many
+  float* part;           // [n, hq, npiece, D + 2]
+  int64_t n;
+  int hq, g, shift, npiece, chunk, window;
+  float scale_log2;
+  bool zero_rest;
+};
+
+constexpr int kPagedPad = 4;  // floats between the rows of an LDS block of partial outputs
+
+// The rows of sequence b.
+struct PagedSeq {
+  int64_t lo;   // first token
+  int nq, len;  // new tokens, keys
+  __device__ __forceinline__ PagedSeq(const PagedArgs& a, int b) {
+    lo = max(0, a.c.cu[b]);
+    nq = (int)(min((int64_t)a.c.cu[b + 1], a.n) - lo);
+    len = min(max(a.c.lens[b], 0), a.c.table_width << a.shift);
+  }
+};
+
+// Keys [lo, hi) that positions [pmin, pmax] see of piece pc.
+__device__ __forceinline__ void paged_range(const PagedArgs& a, int len, int pmin, int pmax, int pc, int& lo, int& hi) {
+  lo = a.window >= 0 ? max(0, pmin - a.window) : 0;
+  hi = min(len, pmax + 1);
+  if (a.npiece > 1) {
+    lo = max(lo, pc * a.chunk);
+    if (pc < a.npiece - 1) hi = min(hi, (pc + 1) * a.chunk);
+  }
+}
+
+// Page ids of a sequence by its wave: lane l holds entry first + l.
+struct PagedIds {
+  const int32_t* row;
+  int width, first, id;
+  int64_t pages;
+  __device__ __forceinline__ void init(const PagedArgs& a, int b) {
+    row = a.c.table + (int64_t)b * a.c.table_row;
+    width = a.c.table_width;
+    pages = a.c.pages;
+    first = -64;
+    id = -1;
+  }
+  // Entry e (wave-uniform), -1 where it names no page.
+  __device__ __forceinline__ int get(int e) {
+    if (e < first || e >= first + 64) {
+      first = e;
+      const int at = e + (int)(threadIdx.x & 63);
+      id = at < width ? row[at] : -1;
+      if (id >= pages) id = -1;
+    }
+    return max(__builtin_amdgcn_readlane(id, e - first), -1);
+  }
+};
+
+// Copies of one kv head's rows into a kSwz tile, ROWS (8 or 16) at a time: rows row0
+// .. row0 + ROWS - 1 of a 16-key group.
+template <int D, int ROWS = 16>
+struct PagedDma {
+  static constexpr int CH = D / 8, RPB = 64 / CH, BLOCKS = ROWS / RPB;
+  using Geo = TileGeom<D, kSwz>;
+  const bf16* base;
+  int64_t page_stride;
+  int slot_stride;
+  uint32_t o[BLOCKS];
+  __device__ __forceinline__ void init(const void* pages, int64_t page, int64_t head, int64_t slot, int h, int row0 = 0) {
+    base = static_cast<const bf16*>(pages) + h * head;
+    page_stride = page;
+    slot_stride = (int)slot;
+    const int j = threadIdx.x & 63;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      const int row = RPB * b + j / CH;  // the swizzle has period 16
+      o[b] = (uint32_t)(row * slot_stride + 8 * ((j % CH) ^ Geo::swz(row0 + row))) * 2u;
+    }
+  }
+  // `rows` valid rows (none or less: zeros) from slot `slot` of page `page` (negative: zeros) on, to dst
+  __device__ __forceinline__ void issue(bf16* dst, int page, int slot, int rows) const {
+    const bf16* p = base + (int64_t)max(page, 0) * page_stride + (int64_t)slot * slot_stride;
+    const int bytes = rows > 0 && page >= 0 ? ((min(rows, ROWS) - 1) * slot_stride + D) * 2 : 0;
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(p), (short)0, bytes, kBufRsrcWord3);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) buf_load_lds16(r, dst + RPB * b * D, o[b]);
+  }
+};
+
+// Whether all values of `steps` 16-key steps of a V tile are finite: their products
+// with zero, which are NaN for the others, summed by the matrix unit.
+template <typename EL, int D, int STEPS>
+__device__ __forceinline__ bool paged_tile_finite(const TileReader<D, kSwz>& rd, const bf16* vt) {
+  using E8 = typename Elem<EL>::x8;
+  f32x16 z = f32x16{};
+#pragma unroll
+  for (int ks = 0; ks < STEPS; ++ks)
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) z = mfma32(rd.template tr<EL>(vt, 16 * ks, dt), E8{}, z);
+  float t = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) t += z[e];
+  return __ballot(t != t) == 0;
+}
+
+// O += V^T P over one 16-key step whose values may be infinite or NaN: those count
+// as zero, and elements of rows that see one become NaN.  seen: bit e, whether the
+// row sees the lane's key e of the step.
+template <typename EL, int D>
+__device__ __forceinline__ void paged_pv_guarded(f32x16 (&oacc)[D / 32], const TileReader<D, kSwz>& rd, const bf16* vt,
+                                                 int ks, const typename Elem<EL>::x8 pb, uint32_t seen) {
+  using E8 = typename Elem<EL>::x8;
+  E8 sees;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sees[e] = (EL)(seen >> e & 1 ? 1.f : 0.f);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) {
+    const E8 v = rd.template tr<EL>(vt, 16 * ks, dt);
+    E8 fin, odd;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool ok = fabsf((float)v[e]) < INFINITY;
+      fin[e] = ok ? v[e] : (EL)0.f;
+      odd[e] = (EL)(ok ? 0.f : 1.f);
+    }
+    oacc[dt] = mfma32(fin, pb, oacc[dt]);
+    const f32x16 bad = mfma32(odd, sees, f32x16{});
+#pragma unroll
+    for (int e = 0; e < 16; ++e) oacc[dt][e] = bad[e] > 0.f ? __builtin_nanf("") : oacc[dt][e];
+  }
+}
+
+// Sequence that token n belongs to, or nseq.  By a whole wave.
+__device__ __forceinline__ int paged_seq_of(const int32_t* cu, int nseq, int64_t n) {
+  const int lane = threadIdx.x & 63;
+  int cnt = 0;  // ends at or before n
+  for (int c = 0; c < nseq; c += 64) {
+    const bool past = c + lane < nseq && (int64_t)cu[c + lane + 1] <= n;
+    cnt += __builtin_popcountll(__ballot(past));
+  }
+  return cnt;
+}
+
+// The launcher of the kernel for chunks of many rows (paged_tile.hip), and the rows
+// that one of its workgroups takes.
+int paged_launch_tile(const PagedArgs& a, int h, int d, bool half, hipStream_t st);
+constexpr int kTileRows = 128;
 
 }  // namespace logo

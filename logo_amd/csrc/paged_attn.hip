@@ -28,139 +28,6 @@
 
 namespace logo {
 
-struct PagedArgs {
-  logo_paged_cache c;
-  const bf16* q;
-  int64_t q_token, q_head;
-  bf16* out;             // [n, hq, D]
-  const uint8_t* sel;    // [n] or null: every token
-  float* part;           // [n, hq, npiece, D + 2]
-  int64_t n;
-  int hq, g, shift, npiece, chunk, window;
-  float scale_log2;
-  bool zero_rest;
-};
-
-constexpr int kPagedPad = 4;  // floats between the rows of an LDS block of partial outputs
-
-// The rows of sequence b.
-struct PagedSeq {
-  int64_t lo;   // first token
-  int nq, len;  // new tokens, keys
-  __device__ __forceinline__ PagedSeq(const PagedArgs& a, int b) {
-    lo = max(0, a.c.cu[b]);
-    nq = (int)(min((int64_t)a.c.cu[b + 1], a.n) - lo);
-    len = min(max(a.c.lens[b], 0), a.c.table_width << a.shift);
-  }
-};
-
-// Keys [lo, hi) that positions [pmin, pmax] see of piece pc.
-__device__ __forceinline__ void paged_range(const PagedArgs& a, int len, int pmin, int pmax, int pc, int& lo, int& hi) {
-  lo = a.window >= 0 ? max(0, pmin - a.window) : 0;
-  hi = min(len, pmax + 1);
-  if (a.npiece > 1) {
-    lo = max(lo, pc * a.chunk);
-    if (pc < a.npiece - 1) hi = min(hi, (pc + 1) * a.chunk);
-  }
-}
-
-// Page ids of a sequence by its wave: lane l holds entry first + l.
-struct PagedIds {
-  const int32_t* row;
-  int width, first, id;
-  int64_t pages;
-  __device__ __forceinline__ void init(const PagedArgs& a, int b) {
-    row = a.c.table + (int64_t)b * a.c.table_row;
-    width = a.c.table_width;
-    pages = a.c.pages;
-    first = -64;
-    id = -1;
-  }
-  // Entry e (wave-uniform), -1 where it names no page.
-  __device__ __forceinline__ int get(int e) {
-    if (e < first || e >= first + 64) {
-      first = e;
-      const int at = e + (int)(threadIdx.x & 63);
-      id = at < width ? row[at] : -1;
-      if (id >= pages) id = -1;
-    }
-    return max(__builtin_amdgcn_readlane(id, e - first), -1);
-  }
-};
-
-// Copies of 16-key groups of one kv head's rows into a kSwz tile.
-template <int D>
-struct PagedDma {
-  static constexpr int CH = D / 8, RPB = 64 / CH, BLOCKS = 16 / RPB;
-  using Geo = TileGeom<D, kSwz>;
-  const bf16* base;
-  int64_t page_stride;
-  int slot_stride;
-  uint32_t o[BLOCKS];
-  __device__ __forceinline__ void init(const void* pages, int64_t page, int64_t head, int64_t slot, int h) {
-    base = static_cast<const bf16*>(pages) + h * head;
-    page_stride = page;
-    slot_stride = (int)slot;
-    const int j = threadIdx.x & 63;
-#pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
-      const int row = RPB * b + j / CH;  // the swizzle has period 16
-      o[b] = (uint32_t)(row * slot_stride + 8 * ((j % CH) ^ Geo::swz(row))) * 2u;
-    }
-  }
-  // `rows` valid rows (at most 16; none: zeros) from slot `slot` of page `page` to tile rows 0 .. 15 of dst
-  __device__ __forceinline__ void issue(bf16* dst, int page, int slot, int rows) const {
-    const bf16* p = base + (int64_t)max(page, 0) * page_stride + (int64_t)slot * slot_stride;
-    const int bytes = rows > 0 && page >= 0 ? ((min(rows, 16) - 1) * slot_stride + D) * 2 : 0;
-    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(p), (short)0, bytes, kBufRsrcWord3);
-#pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) buf_load_lds16(r, dst + RPB * b * D, o[b]);
-  }
-};
-
-// Whether all values of `steps` 16-key steps of a V tile are finite: their products
-// with zero, which are NaN for the others, summed by the matrix unit.
-template <typename EL, int D, int STEPS>
-__device__ __forceinline__ bool paged_tile_finite(const TileReader<D, kSwz>& rd, const bf16* vt) {
-  using E8 = typename Elem<EL>::x8;
-  f32x16 z = f32x16{};
-#pragma unroll
-  for (int ks = 0; ks < STEPS; ++ks)
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) z = mfma32(rd.template tr<EL>(vt, 16 * ks, dt), E8{}, z);
-  float t = 0.f;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) t += z[e];
-  return __ballot(t != t) == 0;
-}
-
-// O += V^T P over one 16-key step whose values may be infinite or NaN: those count
-// as zero, and elements of rows that see one become NaN.  seen: bit e, whether the
-// row sees the lane's key e of the step.
-template <typename EL, int D>
-__device__ __forceinline__ void paged_pv_guarded(f32x16 (&oacc)[D / 32], const TileReader<D, kSwz>& rd, const bf16* vt,
-                                                 int ks, const typename Elem<EL>::x8 pb, uint32_t seen) {
-  using E8 = typename Elem<EL>::x8;
-  E8 sees;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sees[e] = (EL)(seen >> e & 1 ? 1.f : 0.f);
-#pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt) {
-    const E8 v = rd.template tr<EL>(vt, 16 * ks, dt);
-    E8 fin, odd;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool ok = fabsf((float)v[e]) < INFINITY;
-      fin[e] = ok ? v[e] : (EL)0.f;
-      odd[e] = (EL)(ok ? 0.f : 1.f);
-    }
-    oacc[dt] = mfma32(fin, pb, oacc[dt]);
-    const f32x16 bad = mfma32(odd, sees, f32x16{});
-#pragma unroll
-    for (int e = 0; e < 16; ++e) oacc[dt][e] = bad[e] > 0.f ? __builtin_nanf("") : oacc[dt][e];
-  }
-}
-
 // ---------------------------------------------------------------------------
 // Few rows
 // ---------------------------------------------------------------------------
@@ -357,16 +224,12 @@ template <typename EL, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   const int64_t row = blockIdx.x, n = row / a.hq;
   const int tid = threadIdx.x, l = tid & 63;
-  int cnt = 0;
-  for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
-    const bool past = b0 + l < a.c.nseq && (int64_t)a.c.cu[b0 + l + 1] <= n;
-    cnt += __builtin_popcountll(__ballot(past));
-  }
-  if (cnt == a.c.nseq || n < a.c.cu[cnt]) {
+  const int b = paged_seq_of(a.c.cu, a.c.nseq, n);
+  if (b == a.c.nseq || n < a.c.cu[b]) {
     if (a.zero_rest && tid < D / 8) reinterpret_cast<u32x4*>(a.out + row * D)[tid] = u32x4{};
     return;
   }
-  const PagedSeq s(a, cnt);
+  const PagedSeq s(a, b);
   const int p = s.len - s.nq + (int)(n - s.lo);
   const bool valid = p >= 0 && (a.sel == nullptr || a.sel[n] != 0);
   // the pieces that hold keys which the row sees
@@ -406,26 +269,49 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   }
 }
 
+// Whether a call's rows go 32 at a time through the kernel for few rows: where no
+// sequence has more (by the caller's bound; others stay right, 32 after 32).
+static bool paged_few(int max_q, int g) { return (int64_t)max_q * g <= 32; }
+
 // How the keys are cut: pieces per sequence and keys per piece (a multiple of 128).
-static void paged_pieces(int nseq, int h, int max_len, int window, int max_q, int& npiece, int& chunk) {
-  const int64_t wgs = (int64_t)std::max(nseq, 1) * h;
-  const int64_t span = window >= 0 ? std::min<int64_t>(max_len, (int64_t)window + max_q) : max_len;
-  int64_t want = std::min<int64_t>((1024 + wgs - 1) / wgs, (span + 255) / 256);
-  if (window >= 0) want = 1;  // a window's keys are few
-  want = std::max<int64_t>(want, 1);
-  const int64_t per = std::max<int64_t>((max_len + want - 1) / want, 1);
-  chunk = (int)std::min<int64_t>((per + 127) & ~(int64_t)127, (int64_t)1 << 30);
-  npiece = std::max(1, (max_len + chunk - 1) / chunk);
+struct PagedPlan {
+  bool few;
+  int npiece, chunk;
+  size_t part_bytes, bytes;
+};
+
+static PagedPlan paged_plan(int nseq, int h, int hq, int64_t n, int d, int max_q, int max_len, int window, bool sel) {
+  PagedPlan p{};
+  const int g = hq / h;
+  p.few = paged_few(max_q, g);
+  max_len = std::max(max_len, 1);
+  int64_t want = 1;
+  if (window < 0) {  // a window's keys are few
+    const int64_t wgs = (p.few ? (int64_t)nseq : n * g / kTileRows + nseq) * h;
+    if (p.few) want = std::min<int64_t>((1024 + wgs - 1) / wgs, (max_len + 255) / 256);
+    else if (wgs < 384) want = std::min<int64_t>((1024 + wgs - 1) / wgs, (max_len + 511) / 512);
+  }
+  const int64_t per = (max_len + want - 1) / want;
+  p.chunk = (int)std::min<int64_t>((per + 127) & ~(int64_t)127, (int64_t)1 << 30);
+  p.npiece = (max_len + p.chunk - 1) / p.chunk;
+  if (p.npiece > 1) p.part_bytes = ((size_t)n * hq * p.npiece * (d + 2) * sizeof(float) + 255) & ~(size_t)255;
+  p.bytes = p.part_bytes + (sel && !p.few ? ((size_t)n + nseq) * sizeof(int32_t) : 0);
+  return p;
 }
 
 template <typename EL, int D>
-static int paged_launch(const PagedArgs& a, int h, hipStream_t st) {
-  auto few = paged_few_kernel<EL, D>;
-  LOGO_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(few), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)few_smem<D>()));
-  const bool rest = a.npiece == 1 && a.zero_rest;
-  hipLaunchKernelGGL(few, dim3(a.npiece, h, a.c.nseq + (rest ? 1 : 0)), dim3(64 * kFewWaves), few_smem<D>(), st, a);
-  LOGO_LAUNCH_CHECK("paged_few_kernel");
+static int paged_launch(const PagedArgs& a, bool few, int h, hipStream_t st) {
+  if (few) {
+    auto kern = paged_few_kernel<EL, D>;
+    LOGO_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<D>()));
+    const bool rest = a.npiece == 1 && a.zero_rest;
+    hipLaunchKernelGGL(kern, dim3(a.npiece, h, a.c.nseq + (rest ? 1 : 0)), dim3(64 * kFewWaves), few_smem<D>(), st, a);
+    LOGO_LAUNCH_CHECK("paged_few_kernel");
+  } else {
+    const int rc = paged_launch_tile(a, h, D, Elem<EL>::kHalf, st);
+    if (rc != LOGO_OK) return rc;
+  }
   if (a.npiece > 1) {
     hipLaunchKernelGGL((paged_join_kernel<EL, D>), dim3((unsigned)(a.n * a.hq)), dim3(256), 0, st, a);
     LOGO_LAUNCH_CHECK("paged_join_kernel");
@@ -438,11 +324,9 @@ static int paged_launch(const PagedArgs& a, int h, hipStream_t st) {
 using namespace logo;
 
 extern "C" size_t logo_paged_attn_workspace_bytes(int nseq, int h, int hq, int64_t n_tokens, int d, int max_q,
-                                                  int max_len, int window) {
-  if (nseq < 1 || h < 1 || hq < 1 || n_tokens < 1 || max_len < 1) return 0;
-  int npiece, chunk;
-  paged_pieces(nseq, h, max_len, window, max_q, npiece, chunk);
-  return npiece > 1 ? (size_t)n_tokens * hq * npiece * (d + 2) * sizeof(float) : 0;
+                                                  int max_len, int window, int selected) {
+  if (nseq < 1 || h < 1 || hq < h || n_tokens < 1) return 0;
+  return paged_plan(nseq, h, hq, n_tokens, d, max_q, max_len, window, selected != 0).bytes;
 }
 
 extern "C" int logo_paged_attn(const logo_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head, void* out,
@@ -476,11 +360,16 @@ extern "C" int logo_paged_attn(const logo_paged_cache* cache, const void* q, int
   a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.zero_rest = zero_rest != 0;
-  paged_pieces(a.c.nseq, h, std::max(1, max_len), window, max_q, a.npiece, a.chunk);
-  const size_t need = logo_paged_attn_workspace_bytes(a.c.nseq, h, hq, n_tokens, d, max_q, max_len, window);
-  LOGO_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "the workspace is too small");
+  const PagedPlan plan = paged_plan(std::max(a.c.nseq, 1), h, hq, n_tokens, d, max_q, max_len, window, selection != nullptr);
+  LOGO_REQUIRE(a.c.nseq == 0 || plan.bytes == 0 || (workspace != nullptr && workspace_bytes >= plan.bytes),
+               "the workspace is too small");
+  a.npiece = a.c.nseq == 0 ? 1 : plan.npiece;
+  a.chunk = plan.chunk;
   a.part = static_cast<float*>(workspace);
+  a.idx = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + plan.part_bytes);
+  a.count = a.idx + n_tokens;
+  const bool few = plan.few || a.c.nseq == 0;
   hipStream_t st = as_stream(stream);
-  if (dtype == LOGO_DTYPE_BF16) return d == 128 ? paged_launch<bf16, 128>(a, h, st) : paged_launch<bf16, 64>(a, h, st);
-  return d == 128 ? paged_launch<f16, 128>(a, h, st) : paged_launch<f16, 64>(a, h, st);
+  if (dtype == LOGO_DTYPE_BF16) return d == 128 ? paged_launch<bf16, 128>(a, few, h, st) : paged_launch<bf16, 64>(a, few, h, st);
+  return d == 128 ? paged_launch<f16, 128>(a, few, h, st) : paged_launch<f16, 64>(a, few, h, st);
 }

@@ -86,18 +86,6 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t frac) {
   return float2{negc ? -cs : cs, negs ? -sn : sn};
 }
 
-// Number of ends cu[1 .. nseq] at or before token n: its sequence, nseq behind
-// the last one.  By a whole wave, 64 sequences a step.
-__device__ __forceinline__ int wave_seq_of(const int32_t* cu, int nseq, int64_t n) {
-  const int lane = threadIdx.x & 63;
-  int cnt = 0;
-  for (int c = 0; c < nseq; c += 64) {
-    const bool past = c + lane < nseq && (int64_t)cu[c + lane + 1] <= n;
-    cnt += __builtin_popcountll(__ballot(past));
-  }
-  return cnt;
-}
-
 // What a workgroup knows of each of its tokens.
 struct RotTok {
   int64_t pos;    // position
@@ -120,7 +108,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(const RotArgs a) {
   if constexpr (APPEND) {
     for (int t = tid >> 6; t < ntok; t += kRotThreads / 64) {
       const int64_t n = n0 + t;
-      const int b = wave_seq_of(a.cu, a.nseq, n);
+      const int b = paged_seq_of(a.cu, a.nseq, n);
       RotTok k{0, n * r.x_token, n * r.y_token, 1};
       if (b < a.nseq) {
         const int lo = a.cu[b], hi = a.cu[b + 1];

@@ -182,7 +182,8 @@ def paged_attn(q, k_pages, v_pages, block_table, cu_seqlens, lens, max_q: Option
     window = min(int(window), (1 << 31) - 1)
     q = _rows16(q)
     lib = _lib.lib()
-    nbytes = lib.logo_paged_attn_workspace_bytes(c.nseq, H, HQ, N, D, max_q, max_len, window)
+    nbytes = lib.logo_paged_attn_workspace_bytes(c.nseq, H, HQ, N, D, max_q, max_len, window,
+                                                 selection is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     with _lib.on_device(k_pages):
         _lib.launch("logo_paged_attn", lib.logo_paged_attn, c, _lib.ptr(q), *_strides(q), _lib.ptr(out),
