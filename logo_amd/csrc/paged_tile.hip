@@ -12,8 +12,6 @@
 
 namespace logo {
 
-constexpr int kTileWaves = kTileRows / 32;
-
 template <int D>
 constexpr size_t tile_smem() { return (size_t)4 * 64 * D * sizeof(bf16); }  // K and V, two of each
 
@@ -57,7 +55,7 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedAr
 // one kv head: the rank-th of them.  By a whole wave.
 struct TileWork {
   int b, tile, piece, rows;
-  __device__ __forceinline__ bool find(const PagedArgs& a, int64_t rank) {
+  __device__ __forceinline__ bool find(const PagedArgs& a, int64_t rank, int tile_rows) {
     const int lane = threadIdx.x & 63;
     for (int c = 0; c < a.c.nseq; c += 64) {
       int r = 0;
@@ -65,7 +63,7 @@ struct TileWork {
         const PagedSeq s(a, c + lane);
         r = max(0, a.sel ? a.count[c + lane] : s.nq) * a.g;
       }
-      const int nt = (r + kTileRows - 1) / kTileRows * a.npiece;
+      const int nt = (r + tile_rows - 1) / tile_rows * a.npiece;
       int pre = nt;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
@@ -89,12 +87,68 @@ struct TileWork {
   }
 };
 
-template <typename EL, int D, bool WINDOW>
-__global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// Page ids of the rows that a wave copies, for 64 tiles at a time (lane l: tile
+// 64 block + l), and which 16-key groups of those tiles have a page at all.
+struct TilePages {
+  const int32_t* row;
+  int64_t pages;
+  int width, shift, kv_lo, len, own, block, id;
+  unsigned long long ok[4];
+  __device__ __forceinline__ void init(const PagedArgs& a, int b, int lo, int length, int first_row) {
+    row = a.c.table + (int64_t)b * a.c.table_row;
+    pages = a.c.pages;
+    width = a.c.table_width;
+    shift = a.shift;
+    kv_lo = lo;
+    len = length;
+    own = first_row >> 4;
+    block = -1;
+  }
+  // Page of the wave's rows of tile x (negative: none), and in `bad` the groups of the tile without one.
+  __device__ __forceinline__ int get(int x, uint32_t& bad) {
+    if (x >> 6 != block) {
+      block = x >> 6;
+      const int j0 = kv_lo + 64 * (64 * block + (int)(threadIdx.x & 63));
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + 16 * u, e = j >> shift;
+        int v = -1;
+        if (j < len && e < width) v = row[e];
+        const bool held = v >= 0 && v < pages;
+        ok[u] = __ballot(held || j >= len);  // keys behind the last one are masked by position
+        if (u == own) id = held ? v : -1;
+      }
+    }
+    const int at = x & 63;
+    bad = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) bad |= (ok[u] >> at & 1) ? 0u : 1u << u;
+    return __builtin_amdgcn_readlane(id, at);
+  }
+};
+
+// The loop over key tiles is software-pipelined inside each wave, as in sq_fwd.hip:
+// step t runs the MFMAs of S(t + 1) and of O += V(t)^T P(t) slot by slot, with the
+// exponentials of P(t) spread over the first three quarters of the slots, the mask and
+// row maximum of S(t + 1) over the second half, and operand reads four slots ahead.
+// K is copied one tile further ahead than V.  A row's reference maximum moves only when
+// its maximum grew by more than 2^8 (or on its first key), so O is rarely rescaled.
+template <typename EL, int D, bool WINDOW, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_tile_kernel(const PagedArgs a) {
   using E8 = typename Elem<EL>::x8;
   using E4 = typename Elem<EL>::x4;
-  constexpr int NW = kTileWaves, DS = D / 16, DT = D / 32;
+  constexpr int ROWS = 32 * NW, RPW = 64 / NW, DS = D / 16, DT = D / 32;
+  constexpr int NX = 2 * DS, NY = 4 * DT;     // MFMA slots of S and of PV
+  constexpr int IY = 32 / NY;                 // mask / maximum items per Y slot
+  constexpr int NPS = NX + 3 * DT - 1;        // slots that carry items of P
+  constexpr auto pfirst = [](int s) constexpr { return (32 * s + NPS - 1) / NPS < 32 ? (32 * s + NPS - 1) / NPS : 32; };
+  constexpr auto pslot = [](int it) constexpr { return it * NPS / 32; };
+  constexpr int kMaxPerSlot = (32 + NPS - 1) / NPS;
+  static_assert(pfirst(NPS) == 32 && pslot(7) + 1 < NX && pslot(15) + 1 < NX + DT && pslot(23) + 1 < NX + 2 * DT &&
+                    pslot(31) + 1 < NX + 3 * DT,
+                "each group of eight items of P is packed before its PV MFMAs");
+  constexpr int PF = 4;                       // operand reads, in slots ahead
   using GT = TileGeom<D, kSwz>;
   extern __shared__ __attribute__((aligned(16))) char tile_mem[];
   bf16* const smem = reinterpret_cast<bf16*>(tile_mem);
@@ -118,17 +172,16 @@ void paged_tile_kernel(const PagedArgs a) {
     }
   }
   TileWork w;
-  if (!w.find(a, rank)) return;
+  if (!w.find(a, rank, ROWS)) return;
   const PagedSeq s(a, w.b);
-  const int r0 = w.tile * kTileRows, pos0 = s.len - s.nq;
+  const int r0 = w.tile * ROWS, pos0 = s.len - s.nq;
   // token in the sequence of row r
   auto token = [&](int r) { return a.sel ? a.idx[s.lo + r / a.g] : r / a.g; };
-  const int rl = min(r0 + kTileRows, w.rows) - 1;  // last row
-  const int wr = r0 + 32 * wave, r = wr + i;
-  const bool valid = r <= rl;
-  const int tok = token(min(r, rl));
+  const int rl = min(r0 + ROWS, w.rows) - 1;  // last row
+  const int wr = r0 + 32 * wave, r = min(wr + i, rl);
+  const bool valid = wr + i <= rl, active = wr <= rl;
+  const int tok = token(r), hrow = r % a.g;   // and its query head in the group
   const int p = valid ? pos0 + tok : -1;
-  const bool active = wr <= rl;
   const int pmin = pos0 + __builtin_amdgcn_readfirstlane(token(min(wr, rl)));
   const int pmax = active ? pos0 + __builtin_amdgcn_readfirstlane(token(min(wr + 31, rl))) : -1;
   int kv_lo, kv_hi;
@@ -137,7 +190,6 @@ void paged_tile_kernel(const PagedArgs a) {
   kv_lo &= ~63;
   if (a.npiece > 1 && kv_lo >= kv_hi) return;
   const int W = a.window, nt = max(0, (kv_hi - kv_lo + 63) >> 6);
-  const int hrow = min(r, rl) - min(r, rl) / a.g * a.g;  // query head in the group
 
   E8 qreg[DS];
   {
@@ -148,86 +200,181 @@ void paged_tile_kernel(const PagedArgs a) {
   f32x16 oacc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
-  float m_run = -INFINITY, l_run = 0.f;
+  f32x16 sbuf[2][2];  // [t & 1][32-key half]: scores of this tile and the next
+  E8 pb[4];           // P(t) as the PV MFMAs' operand
+  float m_run = -INFINITY, l_run = 0.f, base = 0.f;
   const float c = a.scale_log2;
 
-  TileReader<D, kSwz> rd;
+  TileReader<D, kSwz> rd;  // K read along rows, V transposed
   rd.init();
-  PagedDma<D> dk, dv;
-  dk.init(a.c.k, a.c.k_page, a.c.k_head, a.c.k_slot, h);
-  dv.init(a.c.v, a.c.v_page, a.c.v_head, a.c.v_slot, h);
-  PagedIds ids;
-  ids.init(a, w.b);
-  auto page_of = [&](int j) { return j < s.len ? ids.get(j >> a.shift) : -1; };
-  auto load = [&](const PagedDma<D>& d, bf16* tile, int t) {
-    const int j = kv_lo + 64 * t + 16 * wave;
-    d.issue(tile + 16 * wave * D, page_of(j), j & ((1 << a.shift) - 1), s.len - j);
+  PagedDma<D, RPW> dk, dv;
+  dk.init(a.c.k, a.c.k_page, a.c.k_head, a.c.k_slot, h, RPW * wave & 15);
+  dv.init(a.c.v, a.c.v_page, a.c.v_head, a.c.v_slot, h, RPW * wave & 15);
+  TilePages pages;
+  pages.init(a, w.b, kv_lo, s.len, RPW * wave);
+  auto load = [&](const PagedDma<D, RPW>& d, bf16* tile, int t, int page) {
+    const int j = kv_lo + 64 * t + RPW * wave;
+    d.issue(tile + RPW * wave * D, page, j & ((1 << a.shift) - 1), s.len - j);
   };
-  // the wave's tiles
-  const int tw_hi = active ? min(nt, ((pmax - kv_lo) >> 6) + 1) : 0;
+  const int tw_hi = active ? min(nt, ((pmax - kv_lo) >> 6) + 1) : 0;  // the wave's tiles
   const int tw_lo = WINDOW && active ? max(0, pmin - W - kv_lo) >> 6 : 0;
-  if (nt > 0) load(dk, tileK(0), 0), load(dv, tileV(0), 0);
-  for (int t = 0; t < nt; ++t) {
-    if (t + 1 < nt) load(dk, tileK((t + 1) & 1), t + 1), load(dv, tileV((t + 1) & 1), t + 1);
-    if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * PagedDma<D>::BLOCKS) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t >= tw_lo && t < tw_hi) {
-      const int j0 = kv_lo + 64 * t;
-      const bf16 *kt = tileK(t & 1), *vt = tileV(t & 1);
-      uint32_t has = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) has |= page_of(j0 + 16 * u) >= 0 ? 1u << u : 0u;
-      f32x16 sc[2];
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        sc[kk] = f32x16{};
-#pragma unroll
-        for (int ds = 0; ds < DS; ++ds) sc[kk] = mfma32(rd.template row<EL>(kt, 32 * kk, ds), qreg[ds], sc[kk]);
-      }
-      uint32_t seen = 0;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = j0 + 32 * kk + rowmap(g, e);
-          const bool vis = key <= p && (!WINDOW || key >= p - W) && (has >> (2 * kk + e / 8) & 1);
-          seen |= vis ? 1u << (16 * kk + e) : 0u;
-          sc[kk][e] = vis ? sc[kk][e] * c : -INFINITY;
-          mx = fmaxf(mx, sc[kk][e]);
-        }
-      const float m_new = fmaxf(m_run, pair_max(mx));
-      const float base = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = fast_exp2(m_run - base);
-      m_run = m_new;
-      float sum = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sc[kk][e] = fast_exp2(sc[kk][e] - base);
-          sum += sc[kk][e];
-        }
-      l_run = l_run * alpha + sum;
-      if (__ballot(alpha != 1.f)) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
-      }
-      if (__ballot(p >= 0 && seen != 0xffffffffu) != 0 && !paged_tile_finite<EL, D, 4>(rd, vt)) {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          paged_pv_guarded<EL, D>(oacc, rd, vt, ks, acc_to<EL>(sc[ks / 2], ks & 1), seen >> (8 * ks));
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const E8 pb = acc_to<EL>(sc[ks / 2], ks & 1);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) oacc[dt] = mfma32(rd.template tr<EL>(vt, 16 * ks, dt), pb, oacc[dt]);
-        }
-      }
+  int page_v = -1;              // page of the wave's rows of tile t + 1
+  uint32_t bad1 = 0, bad2 = 0;  // groups without a page of tiles t + 1 and t + 2
+  bool edge = false;            // tile t crosses the edge of some row's keys
+
+  auto step = [&](auto par_tag, int t) {
+    constexpr int PAR = decltype(par_tag)::value;  // t & 1
+    if (t + 1 < nt) load(dv, tileV(PAR ^ 1), t + 1, page_v);
+    bad1 = bad2;
+    if (t + 2 < nt) {
+      page_v = pages.get(t + 2, bad2);
+      load(dk, tileK(PAR), t + 2, page_v);
     }
+    const bf16* const kb = tileK(PAR ^ 1);
+    const bf16* const vb = tileV(PAR);
+    const int j0n = kv_lo + 64 * (t + 1);
+
+    auto body = [&](auto dos_tag, auto dopv_tag, auto mask_tag) {
+      constexpr bool DOS = decltype(dos_tag)::value;    // S(t + 1) and its statistics
+      constexpr bool DOPV = decltype(dopv_tag)::value;  // P(t) and O += V^T P
+      constexpr bool MASK = decltype(mask_tag)::value;  // S(t + 1) crosses an edge
+      E8 op[NX + NY];
+      auto load_op = [&](auto s_c) {
+        constexpr int S = decltype(s_c)::value;
+        if constexpr (S < NX) {
+          if constexpr (DOS) op[S] = rd.template row<EL>(kb, 32 * (S / DS), S % DS);
+        } else {
+          if constexpr (DOPV) op[S] = rd.template tr<EL>(vb, 16 * ((S - NX) / DT), (S - NX) % DT);
+        }
+      };
+      static_for<PF>([&](auto s_c) { load_op(s_c); });
+      const int hi = p - j0n - 4 * g;  // key offsets in [hi - W, hi] are seen
+      float mx = -INFINITY, psum = 0.f;
+      static_for<NX + NY>([&](auto s_c) {
+        constexpr int S = decltype(s_c)::value;
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int I0 = pfirst(S), NI = pfirst(S + 1) - I0;
+        float spv[kMaxPerSlot];
+        if constexpr (DOPV)
+          static_for<NI>([&](auto i_c) {
+            constexpr int I = decltype(i_c)::value, IT = I0 + I;
+            spv[I] = sbuf[PAR][IT / 16][IT % 16];
+            pin(spv[I]);
+          });
+        if constexpr (S < NX) {
+          if constexpr (DOS) {
+            constexpr int KK = S / DS, DSI = S % DS;
+            const E8 o = op[S];
+            sbuf[PAR ^ 1][KK] = mfma32(o, qreg[DSI], DSI == 0 ? f32x16{} : sbuf[PAR ^ 1][KK]);
+          }
+        } else {
+          constexpr int Y = S - NX;
+          if constexpr (DOPV) {
+            const E8 o = op[S];
+            oacc[Y % DT] = mfma32(o, pb[Y / DT], oacc[Y % DT]);
+          }
+          if constexpr (DOS) {
+            float sv[IY];
+            static_for<IY>([&](auto e_c) {
+              constexpr int E = decltype(e_c)::value, IT = Y * IY + E, KK = IT / 16, JJ = IT % 16;
+              sv[E] = sbuf[PAR ^ 1][KK][JJ];
+              if constexpr (MASK) {
+                pin(sv[E]);
+                constexpr int off = 32 * KK + 8 * (JJ / 4) + (JJ % 4);
+                bool vis = off <= hi && !(bad1 >> (2 * KK + JJ / 8) & 1);
+                if (WINDOW) vis = vis && off >= hi - W;
+                if (!vis) sv[E] = -INFINITY;
+                sbuf[PAR ^ 1][KK][JJ] = sv[E];
+              }
+            });
+#pragma unroll
+            for (int e = 0; e < IY; e += 2) mx = max3_f32(mx, sv[e], sv[e + 1]);
+          }
+        }
+        if constexpr (DOPV) {
+          static_for<NI>([&](auto i_c) {
+            constexpr int I = decltype(i_c)::value, IT = I0 + I;
+            float pv = fast_exp2(fmaf(spv[I], c, -base));
+            pin(pv);
+            sbuf[PAR][IT / 16][IT % 16] = pv;
+          });
+          if constexpr (S >= 1) {
+            constexpr int J0 = pfirst(S - 1), NJ = I0 - J0;
+            static_for<NJ>([&](auto i_c) {
+              constexpr int IT = J0 + decltype(i_c)::value;
+              psum += sbuf[PAR][IT / 16][IT % 16];
+              if constexpr (IT % 8 == 7) pb[IT / 8] = acc_to<EL>(sbuf[PAR][IT / 16], (IT / 8) & 1);
+            });
+            if constexpr (NJ > 0) pin(psum);
+          }
+        }
+        if constexpr (S + PF < NX + NY) load_op(std::integral_constant<int, S + PF>{});
+      });
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (DOPV) l_run += psum;
+      if constexpr (DOS) {
+        const float mxs = pair_max(mx) * c;
+        const bool any_grow = __ballot(mxs - m_run > 8.f);
+        const float m_new = any_grow ? fmaxf(m_run, mxs) : m_run;
+        const float nbase = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = fast_exp2(m_run - nbase);
+        l_run *= alpha;
+        m_run = m_new;
+        base = nbase;
+        if (__ballot(alpha != 1.f)) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
+        }
+      }
+    };
+    using T_ = std::true_type;
+    using F_ = std::false_type;
+    const bool doS = t + 1 >= tw_lo && t + 1 < tw_hi;
+    bool doPV = t >= tw_lo && t < tw_hi;
+    if (doPV && edge && !paged_tile_finite<EL, D, 4>(rd, vb)) {
+      // values that are not finite under a mask: this tile by itself
+      const int hi = p - (j0n - 64) - 4 * g;
+      uint32_t bad0;
+      pages.get(t, bad0);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        uint32_t seen = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int jj = 8 * (ks & 1) + e, off = 32 * (ks / 2) + 8 * (jj / 4) + (jj & 3);
+          const float x = fast_exp2(fmaf(sbuf[PAR][ks / 2][jj], c, -base));
+          sbuf[PAR][ks / 2][jj] = x;
+          l_run += x;
+          if (off <= hi && !(bad0 >> ks & 1) && (!WINDOW || off >= hi - W)) seen |= 1u << e;
+        }
+        paged_pv_guarded<EL, D>(oacc, rd, vb, ks, acc_to<EL>(sbuf[PAR][ks / 2], ks & 1), seen);
+      }
+      doPV = false;
+    }
+    const bool maskn = j0n + 63 > pmin || (WINDOW && j0n < pmax - W) || bad1 != 0;
+    if (doS && doPV) {
+      if (maskn) body(T_{}, T_{}, T_{});
+      else body(T_{}, T_{}, F_{});
+    } else if (doS) {
+      body(T_{}, F_{}, T_{});
+    } else if (doPV) {
+      body(F_{}, T_{}, F_{});
+    }
+    edge = maskn;
+    wait_vmem();
     __syncthreads();
+  };
+
+  if (nt > 0) {
+    page_v = pages.get(0, bad2);
+    load(dk, tileK(0), 0, page_v);
+    wait_vmem();
+    __syncthreads();
+    // step -1 copies V(0) and K(1)
+    for (int t = -1; t < nt; t += 2) {
+      step(std::integral_constant<int, 1>{}, t);
+      if (t + 1 < nt) step(std::integral_constant<int, 0>{}, t + 1);
+    }
   }
   const float l_tot = pair_sum(l_run);
   if (a.npiece > 1) {
@@ -264,26 +411,35 @@ void paged_tile_kernel(const PagedArgs a) {
   }
 }
 
-template <typename EL, int D>
+template <typename EL, int D, int NW>
 static int tile_launch(const PagedArgs& a, int h, hipStream_t st) {
   if (a.sel != nullptr) {
     hipLaunchKernelGGL(paged_select_kernel, dim3(a.c.nseq), dim3(kSelThreads), 0, st, a);
     LOGO_LAUNCH_CHECK("paged_select_kernel");
   }
   // each sequence may end inside a tile
-  const int64_t tiles = a.n * a.g / kTileRows + a.c.nseq, blocks = tiles * a.npiece * h;
+  const int64_t tiles = a.n * a.g / (32 * NW) + a.c.nseq, blocks = tiles * a.npiece * h;
   LOGO_REQUIRE(blocks < ((int64_t)1 << 31), "grid too large");
-  auto kern = a.window >= 0 ? paged_tile_kernel<EL, D, true> : paged_tile_kernel<EL, D, false>;
+  auto kern = a.window >= 0 ? paged_tile_kernel<EL, D, true, NW> : paged_tile_kernel<EL, D, false, NW>;
   LOGO_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)tile_smem<D>()));
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(64 * kTileWaves), tile_smem<D>(), st, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(64 * NW), tile_smem<D>(), st, a);
   LOGO_LAUNCH_CHECK("paged_tile_kernel");
   return LOGO_OK;
 }
 
+template <typename EL, int D>
+static int tile_dispatch(const PagedArgs& a, int h, hipStream_t st) {
+#ifdef PAGED_NW8
+  return tile_launch<EL, D, 8>(a, h, st);
+#else
+  return tile_launch<EL, D, 4>(a, h, st);
+#endif
+}
+
 int paged_launch_tile(const PagedArgs& a, int h, int d, bool half, hipStream_t st) {
-  if (half) return d == 128 ? tile_launch<f16, 128>(a, h, st) : tile_launch<f16, 64>(a, h, st);
-  return d == 128 ? tile_launch<bf16, 128>(a, h, st) : tile_launch<bf16, 64>(a, h, st);
+  if (half) return d == 128 ? tile_dispatch<f16, 128>(a, h, st) : tile_dispatch<f16, 64>(a, h, st);
+  return d == 128 ? tile_dispatch<bf16, 128>(a, h, st) : tile_dispatch<bf16, 64>(a, h, st);
 }
 
 }  // namespace logo
