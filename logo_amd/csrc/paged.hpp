@@ -17,7 +17,7 @@ inline int paged_check(const logo_paged_cache* c, int d) {
                "page_size (%d) must be a power of two in [16, 65536]", c->page_size);
   LOGO_REQUIRE(c->nseq >= 0 && c->table_width >= 0 && c->pages >= 0 && c->table_row >= c->table_width,
                "bad sequence, table or page counts");
-  LOGO_REQUIRE((int64_t)c->table_width * c->page_size < ((int64_t)1 << 31), "a sequence must stay below 2^31 keys");
+  LOGO_REQUIRE((int64_t)c->table_width * c->page_size <= ((int64_t)1 << 30), "a sequence must stay within 2^30 keys");
   const int64_t strides[6] = {c->k_page, c->k_head, c->k_slot, c->v_page, c->v_head, c->v_slot};
   for (int64_t s : strides) LOGO_REQUIRE(s % 8 == 0 && s >= 0, "page strides must be multiples of 8 elements");
   // a page's rows are addressed by 32-bit byte offsets
@@ -36,16 +36,27 @@ struct PagedArgs {
   int64_t q_token, q_head;
   bf16* out;             // [n, hq, D]
   const uint8_t* sel;    // [n] or null: every token
-  int32_t* idx;          // [n] with sel: the selected tokens of each sequence, from its first token's place on
-  int32_t* count;        // [nseq] with sel: how many
-  float* part;           // [n, hq, npiece, D + 2]
+  int32_t* idx;          // [n] with sel (many rows): the selected tokens of each sequence, from its first token's place on
+  int32_t* count;        // [nseq] with sel (many rows): how many
+  float* part;           // partial results, D + 2 floats a row (O unnormalised, its reference maximum, its sum)
   int64_t n;
-  int hq, g, shift, npiece, chunk, window;
+  int hq, g, shift, window;
   float scale_log2;
   bool zero_rest;
+  bool split;            // a sequence's keys may be cut into pieces
+  int target;            // workgroups the device holds at once
+  int cap;               // many rows: pieces per kv head that part holds
+  int part_rows;         // rows of a piece in part
 };
 
 constexpr int kPagedPad = 4;  // floats between the rows of an LDS block of partial outputs
+
+// Compute units of the current device (cached per device).
+int device_cus();
+
+// A value that all lanes of the wave hold, as a scalar: what is derived from it (buffer
+// descriptors above all) then stays in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // The rows of sequence b.
 struct PagedSeq {
@@ -53,42 +64,8 @@ struct PagedSeq {
   int nq, len;  // new tokens, keys
   __device__ __forceinline__ PagedSeq(const PagedArgs& a, int b) {
     lo = max(0, a.c.cu[b]);
-    nq = (int)(min((int64_t)a.c.cu[b + 1], a.n) - lo);
+    nq = (int)max((int64_t)0, min((int64_t)a.c.cu[b + 1], a.n) - lo);
     len = min(max(a.c.lens[b], 0), a.c.table_width << a.shift);
-  }
-};
-
-// Keys [lo, hi) that positions [pmin, pmax] see of piece pc.
-__device__ __forceinline__ void paged_range(const PagedArgs& a, int len, int pmin, int pmax, int pc, int& lo, int& hi) {
-  lo = a.window >= 0 ? max(0, pmin - a.window) : 0;
-  hi = min(len, pmax + 1);
-  if (a.npiece > 1) {
-    lo = max(lo, pc * a.chunk);
-    if (pc < a.npiece - 1) hi = min(hi, (pc + 1) * a.chunk);
-  }
-}
-
-// Page ids of a sequence by its wave: lane l holds entry first + l.
-struct PagedIds {
-  const int32_t* row;
-  int width, first, id;
-  int64_t pages;
-  __device__ __forceinline__ void init(const PagedArgs& a, int b) {
-    row = a.c.table + (int64_t)b * a.c.table_row;
-    width = a.c.table_width;
-    pages = a.c.pages;
-    first = -64;
-    id = -1;
-  }
-  // Entry e (wave-uniform), -1 where it names no page.
-  __device__ __forceinline__ int get(int e) {
-    if (e < first || e >= first + 64) {
-      first = e;
-      const int at = e + (int)(threadIdx.x & 63);
-      id = at < width ? row[at] : -1;
-      if (id >= pages) id = -1;
-    }
-    return max(__builtin_amdgcn_readlane(id, e - first), -1);
   }
 };
 
@@ -177,9 +154,10 @@ __device__ __forceinline__ int paged_seq_of(const int32_t* cu, int nseq, int64_t
   return cnt;
 }
 
-// The launcher of the kernel for chunks of many rows (paged_tile.hip), and the rows
-// that one of its workgroups takes.
-int paged_launch_tile(const PagedArgs& a, int h, int d, bool half, hipStream_t st);
-constexpr int kTileRows = 128;
+// The kernel for chunks of many rows (paged_tile.hip): how a call of n tokens that see
+// at most `span` keys each is cut, and its launcher (nw: waves of a workgroup, 32 rows each).
+void tile_plan(int nseq, int h, int g, int64_t n, int64_t span, int cus, bool sel, bool& split, int& target, int& cap,
+               int& nw);
+int paged_launch_tile(const PagedArgs& a, int h, int d, bool half, int nw, hipStream_t st);
 
 }  // namespace logo

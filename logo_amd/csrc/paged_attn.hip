@@ -31,217 +31,352 @@ namespace logo {
 // ---------------------------------------------------------------------------
 // Few rows
 // ---------------------------------------------------------------------------
-// A workgroup takes one piece of a sequence's keys for one kv head; its rows are
-// (token, query head of the group) pairs, 32 at a time.  The four waves split the
-// keys in tiles of 32, each with a double-buffered K and V tile of its own and no
-// barrier in the loop, and join at the end through LDS.
-constexpr int kFewWaves = 4;
+// Bound by reading the keys and values once.  A row is a (token, query head of the
+// group) pair of a sequence and kv head.  The workgroups that the device holds at
+// once share out the keys of all sequences and kv heads evenly, whatever the
+// sequences' lengths: laid end to end (in units of 64 keys, kv head by kv head; keys
+// that no selected row sees are left out), each takes an equal stretch, and works it
+// off sequence by sequence.  Every workgroup finds its stretch itself from cu, lens and
+// selection.  A sequence that is cut leaves partial results, which
+// paged_few_join_kernel joins; at most two of a workgroup's sequences are.
+//
+// Its waves split a sequence's keys in tiles of 32, each through a ring of tile slots
+// of its own in LDS (K(0) V(0) K(1) V(1) ...), without a barrier in the loop: a slot is
+// filled again as soon as its tile has been read, so most of a CU's 160 KB of LDS is in
+// flight at any time, which HBM's latency needs.
+#ifndef FEW_WAVES
+#define FEW_WAVES 2
+#endif
+constexpr int kFewWaves = FEW_WAVES;
+constexpr int kFewUnit = 64;      // keys
+constexpr int kFewMinShare = 4;   // units: the shortest stretch, unless a sequence ends
 
 template <int D>
-constexpr size_t few_smem() { return (size_t)kFewWaves * 2 * 2 * 32 * D * sizeof(bf16); }
+constexpr int few_slots() { return D == 128 ? 5 : 10; }
+template <int D>
+constexpr size_t few_smem() { return (size_t)kFewWaves * few_slots<D>() * 32 * D * sizeof(bf16); }
+
+// The sequences laid end to end, and where a stretch lies.
+struct FewCut {
+  int64_t total, share;  // units a kv head; units a workgroup
+  int units, lo, b;      // the located sequence: its units, its first key, its index
+  int64_t start;         // its first unit
+  int own_units, own_lo; // the lane's sequence of the first 64
+
+  // Units of sequence b's keys that some row sees, from key lo on (at least one where it has new tokens).
+  __device__ __forceinline__ static int units_of(const PagedArgs& a, int b, int& lo) {
+    lo = 0;
+    if (b >= a.c.nseq) return 0;
+    const PagedSeq s(a, b);
+    if (s.nq == 0) return 0;
+    if (a.sel != nullptr) {
+      bool any = false;
+      for (int t = 0; t < s.nq && !any; ++t) any = a.sel[s.lo + t] != 0;
+      if (!any) return 1;
+    }
+    if (a.window >= 0) lo = max(0, s.len - s.nq - a.window) & ~(kFewUnit - 1);
+    return max(1, (s.len - lo + kFewUnit - 1) / kFewUnit);
+  }
+  __device__ __forceinline__ static int scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(v, off);
+      if (lane >= off) v += o;
+    }
+    return v;
+  }
+  __device__ __forceinline__ void init(const PagedArgs& a) {
+    const int lane = threadIdx.x & 63;
+    own_units = units_of(a, lane, own_lo);
+    total = __builtin_amdgcn_readlane(scan(own_units), 63);
+    for (int c = 64; c < a.c.nseq; c += 64) {
+      int x;
+      total += __builtin_amdgcn_readlane(scan(units_of(a, c + lane, x)), 63);
+    }
+    share = max((int64_t)kFewMinShare, (total * a.c.heads + a.target - 1) / a.target);
+  }
+  // kv head of unit pos, and the rest
+  __device__ __forceinline__ int head_of(int64_t pos, int64_t& rest) const {
+    const int h = pos >> 32 == 0 && total >> 32 == 0 ? (int)((uint32_t)pos / (uint32_t)total) : (int)(pos / total);
+    rest = pos - h * total;
+    return h;
+  }
+  // The sequence that holds unit `rest` (< total) of a kv head.  By a whole wave.
+  __device__ __forceinline__ void locate(const PagedArgs& a, int64_t rest) {
+    const int lane = threadIdx.x & 63;
+    int64_t base = 0;
+    int n = own_units, first = own_lo;
+    for (int c = 0; c < a.c.nseq; c += 64) {
+      if (c > 0) n = units_of(a, c + lane, first);
+      const int pre = scan(n);
+      const unsigned long long past = __ballot(rest < base + pre);
+      if (past != 0) {
+        const int j = __builtin_ctzll(past);
+        b = c + j;
+        units = __builtin_amdgcn_readlane(n, j);
+        lo = __builtin_amdgcn_readlane(first, j);
+        start = base + __builtin_amdgcn_readlane(pre, j) - units;
+        return;
+      }
+      base += __builtin_amdgcn_readlane(pre, 63);
+    }
+  }
+};
 
 template <typename EL, int D>
 __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void paged_few_kernel(const PagedArgs a) {
   using E8 = typename Elem<EL>::x8;
-  constexpr int DS = D / 16, DT = D / 32, TILE = 32 * D, NISSUE = 2 * 2 * PagedDma<D>::BLOCKS;
-  constexpr int ORS = D + kPagedPad;
+  constexpr int NW = kFewWaves, DS = D / 16, DT = D / 32, TILE = 32 * D, SLOTS = few_slots<D>();
+  constexpr int NI = 2 * PagedDma<D>::BLOCKS;  // copies a slot
+  constexpr int AHEAD = (SLOTS - 1) * NI;      // copies behind the slot that is read
+  constexpr int ORS = D + kPagedPad, CH = D / 8;
+  static_assert(AHEAD < 64, "vmcnt holds 6 bits");
+  static_assert(NW * (32 * ORS + 64) * sizeof(float) <= few_smem<D>(), "the join fits the slots");
   extern __shared__ __attribute__((aligned(16))) char paged_smem[];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 31, g = l >> 5;
-  const int pc = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  if (b == a.c.nseq) {
-    // tokens of no sequence: zero rows of this kv head's group
-    const int64_t end = max(0, a.c.nseq > 0 ? a.c.cu[a.c.nseq] : 0), begin = a.c.nseq > 0 ? a.c.cu[0] : 0;
-    for (int64_t n = pc; n < a.n; n += gridDim.x) {
-      if (n >= begin && n < end) continue;
-      for (int e = tid; e < a.g * D / 8; e += 64 * kFewWaves)
-        reinterpret_cast<u32x4*>(a.out + (n * a.hq + h * a.g) * D)[e] = u32x4{};
-    }
-    return;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), l = tid & 63, i = l & 31, g = l >> 5;
+  const int w = blockIdx.x;
+  if (a.zero_rest) {
+    // tokens of no sequence
+    const int64_t end = a.c.nseq > 0 ? max(0, a.c.cu[a.c.nseq]) : 0, begin = a.c.nseq > 0 ? a.c.cu[0] : 0;
+    const int row = a.hq * CH;
+    for (int64_t n = w; n < begin; n += gridDim.x)
+      for (int e = tid; e < row; e += 64 * NW) reinterpret_cast<u32x4*>(a.out + n * a.hq * D)[e] = u32x4{};
+    for (int64_t n = end + w; n < a.n; n += gridDim.x)
+      for (int e = tid; e < row; e += 64 * NW) reinterpret_cast<u32x4*>(a.out + n * a.hq * D)[e] = u32x4{};
   }
-  const PagedSeq s(a, b);
-  const int rows = s.nq * a.g, pos0 = s.len - s.nq;
-  PagedIds ids;
-  ids.init(a, b);
-  PagedDma<D> dk, dv;
-  dk.init(a.c.k, a.c.k_page, a.c.k_head, a.c.k_slot, h);
-  dv.init(a.c.v, a.c.v_page, a.c.v_head, a.c.v_slot, h);
+  FewCut cut;
+  cut.init(a);
+  int64_t pos = w * cut.share, rest = 0;
+  const int64_t end = min(pos + cut.share, cut.total * a.c.heads);
+  if (pos >= end) return;
+  int h = cut.head_of(pos, rest);
   TileReader<D, kSwz> rd;
   rd.init();
-  bf16* const tiles = reinterpret_cast<bf16*>(paged_smem) + wave * 4 * TILE;  // [stage][K, V]
-  float* const so = reinterpret_cast<float*>(paged_smem);                     // [wave][32][ORS]
-  __shared__ float sm[kFewWaves][32], sl[kFewWaves][32];
+  bf16* const ring = reinterpret_cast<bf16*>(paged_smem) + wave * SLOTS * TILE;
+  float* const so = reinterpret_cast<float*>(paged_smem);  // [wave][32][ORS], then [wave][32] maxima and sums
+  float* const sm = so + NW * 32 * ORS;
+  float* const sl = sm + NW * 32;
   const float c = a.scale_log2;
 
-  for (int r0 = 0; r0 < rows; r0 += 32) {
-    const int r = r0 + i, tok = min(r, rows - 1) / a.g;
-    const bool valid = r < rows && (a.sel == nullptr || a.sel[s.lo + tok] != 0);
-    const int p = valid ? pos0 + tok : -1;
-    // the row block's positions (rows ascend by token)
-    const int pmin = pos0 + r0 / a.g, pmax = pos0 + (min(r0 + 32, rows) - 1) / a.g;
-    int lo, hi;
-    paged_range(a, s.len, pmin, pmax, pc, lo, hi);
-    const bool any = __ballot(valid && p >= 0) != 0;
-    E8 qreg[DS];
-    {
-      const bf16* const qrow = a.q + (s.lo + tok) * a.q_token + (h * a.g + (min(r, rows - 1) - tok * a.g)) * a.q_head + 8 * g;
+  for (int n; pos < end; pos += n, rest += n) {
+    if (rest == cut.total) ++h, rest = 0;
+    cut.locate(a, rest);
+    const int f = (int)(rest - cut.start);  // units of the sequence before this stretch
+    n = (int)min((int64_t)(cut.units - f), end - pos);
+    const int b = uniform(cut.b);
+    const PagedSeq s(a, b);
+    const int rows = s.nq * a.g, pos0 = s.len - s.nq;
+    // not cut (also where nothing joins: keys or rows beyond the caller's bounds): all of it where it starts
+    const bool whole = n == cut.units || !a.split || rows > a.part_rows;
+    if (whole && f > 0) continue;
+    const int lo = cut.lo + kFewUnit * f, hi_piece = whole ? s.len : min(s.len, lo + kFewUnit * n);
+    PagedDma<D> dk, dv;
+    dk.init(a.c.k, a.c.k_page, a.c.k_head, a.c.k_slot, h);
+    dv.init(a.c.v, a.c.v_page, a.c.v_head, a.c.v_slot, h);
+    // the table read through the scalar cache, whose waits leave the copies alone
+    typedef const __attribute__((address_space(4))) int32_t* Table;
+    const Table table = (Table)(uintptr_t)(a.c.table + (int64_t)b * a.c.table_row);
+
+    for (int r0 = 0; r0 < rows; r0 += 32) {  // 32 rows at a time
+      const int r = min(r0 + i, rows - 1), tok = r / a.g;
+      const bool valid = r0 + i < rows && (a.sel == nullptr || a.sel[s.lo + tok] != 0);
+      const int p = valid ? pos0 + tok : -1;
+      const int pmin = pos0 + r0 / a.g, pmax = pos0 + (min(r0 + 32, rows) - 1) / a.g;
+      const int hi = min(hi_piece, pmax + 1);
+      E8 qreg[DS];
+      {
+        const bf16* const qrow = a.q + (s.lo + tok) * a.q_token + (h * a.g + (r - tok * a.g)) * a.q_head + 8 * g;
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds) qreg[ds] = valid ? *reinterpret_cast<const E8*>(qrow + 16 * ds) : E8{};
-    }
-    f32x16 oacc[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
-    float m_run = -INFINITY, l_run = 0.f;
-    const int first = (lo & ~31) + 32 * wave;
-    const int nt = any && first < hi ? (hi - first + 32 * kFewWaves - 1) / (32 * kFewWaves) : 0;
-    uint32_t held = 0;  // bits 2 k, 2 k + 1: the groups of the tile in stage k have a page
-    auto issue = [&](int t) {
-      const int j0 = first + 32 * kFewWaves * t;
-      bf16* const kt = tiles + (t & 1) * 2 * TILE;
-      held &= ~(3u << (2 * (t & 1)));
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int j = j0 + 16 * u, rem = s.len - j;
-        const int page = rem > 0 ? ids.get(j >> a.shift) : -1, slot = j & ((1 << a.shift) - 1);
-        if (page >= 0) held |= 1u << (2 * (t & 1) + u);
-        dk.issue(kt + 16 * u * D, page, slot, rem);
-        dv.issue(kt + TILE + 16 * u * D, page, slot, rem);
+        for (int ds = 0; ds < DS; ++ds) qreg[ds] = valid ? *reinterpret_cast<const E8*>(qrow + 16 * ds) : E8{};
       }
-    };
-    if (nt > 0) issue(0);
-    for (int t = 0; t < nt; ++t) {
-      if (t + 1 < nt) {
-        // the tile's last reads are done before its copies overwrite it
+      f32x16 oacc[DT];
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
+      float m_run = -INFINITY, l_run = 0.f;
+      const int first = lo + 32 * wave;
+      const int nt = __ballot(p >= 0) != 0 && first < hi ? (hi - first + 32 * NW - 1) / (32 * NW) : 0;
+      int page[2];        // of the groups of the tile whose copies go out next
+      uint32_t held = 0;  // bits 2 (t % 16) + u: group u of tile t has a page
+      auto look_up = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          page[u] = table[min((first + 32 * NW * min(t, nt - 1) + 16 * u) >> a.shift, a.c.table_width - 1)];
+      };
+      // K of tile t, then V of it; past the last tile nothing is read, and the count of copies in flight stays
+      auto issue = [&](const PagedDma<D>& d, bf16* slot, int t, bool is_v) {
+        const int j0 = first + 32 * NW * t;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int j = j0 + 16 * u;
+          const bool has = page[u] >= 0 && page[u] < a.c.pages;
+          const uint32_t bit = 1u << (2 * (t & 15) + u);
+          held = has ? held | bit : held & ~bit;
+          d.issue(slot + 16 * u * D, has ? page[u] : -1, j & ((1 << a.shift) - 1), t < nt ? s.len - j : 0);
+        }
+        if (is_v) look_up(t + 1);
+      };
+      if (nt > 0) {
+        look_up(0);
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) issue(k & 1 ? dv : dk, ring + k * TILE, k / 2, k & 1);
+      }
+      // q has arrived here: waited for inside the loop, it would drain the copies each time
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) pin(qreg[ds]);
+      int at = 0;  // ring slot of the tile that is read next
+      for (int t = 0; t < nt; ++t) {
+        const int j0 = first + 32 * NW * t;
+        const uint32_t has = held >> (2 * (t & 15)) & 3;
+        const bf16* const kt = ring + at * TILE;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(AHEAD) : "memory");
+        // all reads of the tile in flight at once; they are done before its slot's next copies
+        E8 op[2 * DT > DS ? 2 * DT : DS];
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) op[ds] = rd.template row<EL>(kt, 0, ds);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        issue(t + 1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(NISSUE) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 sc = f32x16{};
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) sc = mfma32(op[ds], qreg[ds], sc);
+        // slot 2 t + SLOTS takes the place of K(t): a V where the ring is odd
+        issue(SLOTS & 1 ? dv : dk, ring + at * TILE, t + SLOTS / 2, SLOTS & 1);
+        at = at + 1 == SLOTS ? 0 : at + 1;
+        // V(t), read while S turns into P
+        const bf16* const vt = ring + at * TILE;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(AHEAD) : "memory");
+#pragma unroll
+        for (int k = 0; k < 2 * DT; ++k) op[k] = rd.template tr<EL>(vt, 16 * (k / DT), k % DT);
+        __builtin_amdgcn_sched_barrier(0);
+        float mx = -INFINITY;
+        uint32_t seen = 0xffffu;
+        if (j0 + 31 > pmin || a.window >= 0 || has != 3 || !valid) {
+          seen = 0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = j0 + rowmap(g, e);
+            const bool vis = key <= p && (a.window < 0 || key >= p - a.window) && (has >> (e >> 3) & 1);
+            seen |= vis ? 1u << e : 0u;
+            sc[e] = vis ? sc[e] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+        const float m_new = fmaxf(m_run, pair_max(mx) * c);
+        const float base = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = fast_exp2(m_run - base);
+        m_run = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          sc[e] = fast_exp2(fmaf(sc[e], c, -base));
+          sum += sc[e];
+        }
+        l_run = l_run * alpha + sum;
+        if (__ballot(alpha != 1.f)) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
+        }
+        // rows that are not written (p = -1) need no care
+        const bool edge = __ballot(p >= 0 && seen != 0xffffu) != 0;
+        if (edge && !paged_tile_finite<EL, D, 2>(rd, vt)) {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+            paged_pv_guarded<EL, D>(oacc, rd, vt, ks, acc_to<EL>(sc, ks), seen >> (8 * ks));
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const E8 pb = acc_to<EL>(sc, ks);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) oacc[dt] = mfma32(op[DT * ks + dt], pb, oacc[dt]);
+          }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        issue(SLOTS & 1 ? dk : dv, ring + at * TILE, t + (SLOTS + 1) / 2, !(SLOTS & 1));
+        at = at + 1 == SLOTS ? 0 : at + 1;
       }
-      const int j0 = first + 32 * kFewWaves * t;
-      const bf16* const kt = tiles + (t & 1) * 2 * TILE;
-      const uint32_t has = held >> (2 * (t & 1)) & 3;
-      f32x16 sc = f32x16{};
+      // join the waves
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const float l_tot = pair_sum(l_run);
+      __syncthreads();  // every wave is done with its slots
+      {
+        float* const orow = so + (wave * 32 + i) * ORS;
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds) sc = mfma32(rd.template row<EL>(kt, 0, ds), qreg[ds], sc);
-      float mx = -INFINITY;
-      uint32_t seen = 0;
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = j0 + rowmap(g, e);
-        const bool vis = key <= p && (a.window < 0 || key >= p - a.window) && (has >> (e >> 3) & 1);
-        seen |= vis ? 1u << e : 0u;
-        sc[e] = vis ? sc[e] * c : -INFINITY;
-        mx = fmaxf(mx, sc[e]);
+          for (int q4 = 0; q4 < 4; ++q4) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = oacc[dt][4 * q4 + e];
+            *reinterpret_cast<f32x4*>(orow + 32 * dt + 8 * q4 + 4 * g) = v;
+          }
+        if (g == 0) sm[wave * 32 + i] = m_run, sl[wave * 32 + i] = l_tot;
       }
-      const float m_new = fmaxf(m_run, pair_max(mx));
-      const float base = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = fast_exp2(m_run - base);
-      m_run = m_new;
-      float sum = 0.f;
+      __syncthreads();
+      for (int e = tid; e < 32 * CH; e += 64 * NW) {
+        const int rr = e / CH, ch = e % CH;
+        if (r0 + rr >= rows) break;
+        float m = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sc[e] = fast_exp2(sc[e] - base);
-        sum += sc[e];
-      }
-      l_run = l_run * alpha + sum;
-      if (__ballot(alpha != 1.f)) {
+        for (int k = 0; k < NW; ++k) m = fmaxf(m, sm[k * 32 + rr]);
+        const float base = m == -INFINITY ? 0.f : m;
+        float lsum = 0.f, o[8];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
-      }
-      // rows past the block's last (p = -1) see nothing and are not written
-      const bool edge = __ballot(p >= 0 && seen != 0xffffu) != 0;
-      if (edge && !paged_tile_finite<EL, D, 2>(rd, kt + TILE)) {
+        for (int k = 0; k < 8; ++k) o[k] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-          paged_pv_guarded<EL, D>(oacc, rd, kt + TILE, ks, acc_to<EL>(sc, ks), seen >> (8 * ks));
-      } else {
+        for (int wv = 0; wv < NW; ++wv) {
+          const float x = fast_exp2(sm[wv * 32 + rr] - base);
+          lsum = fmaf(x, sl[wv * 32 + rr], lsum);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const E8 pb = acc_to<EL>(sc, ks);
+          for (int k = 0; k < 8; ++k) o[k] = fmaf(x, so[(wv * 32 + rr) * ORS + 8 * ch + k], o[k]);
+        }
+        if (whole) {
+          const int tk = (r0 + rr) / a.g;
+          const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+          E8 v;
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-            oacc[dt] = mfma32(rd.template tr<EL>(kt + TILE, 16 * ks, dt), pb, oacc[dt]);
+          for (int k = 0; k < 8; ++k) v[k] = (EL)(lsum != 0.f ? o[k] * inv : 0.f);
+          *reinterpret_cast<E8*>(a.out + ((s.lo + tk) * a.hq + h * a.g + (r0 + rr - tk * a.g)) * D + 8 * ch) = v;
+        } else {
+          // a stretch has one sequence that started before it and one that goes on behind it at most
+          float* const pp = a.part + ((int64_t)(2 * w + (f == 0 ? 1 : 0)) * a.part_rows + rr) * (D + 2);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) pp[8 * ch + k] = o[k];
+          if (ch == 0) pp[D] = m, pp[D + 1] = lsum;
         }
       }
+      __syncthreads();
     }
-    // join the waves
-    const float l_tot = pair_sum(l_run);
-    __syncthreads();  // every wave is done with its tiles (and with the block before)
-    {
-      float* const orow = so + (wave * 32 + i) * ORS;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = oacc[dt][4 * q4 + e];
-          *reinterpret_cast<f32x4*>(orow + 32 * dt + 8 * q4 + 4 * g) = v;
-        }
-      if (g == 0) sm[wave][i] = m_run, sl[wave][i] = l_tot;
-    }
-    __syncthreads();
-    constexpr int CH = D / 8;
-    for (int e = tid; e < 32 * CH; e += 64 * kFewWaves) {
-      const int rr = e / CH, ch = e % CH;
-      if (r0 + rr >= rows) break;
-      float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) m = fmaxf(m, sm[w][rr]);
-      const float base = m == -INFINITY ? 0.f : m;
-      float lsum = 0.f, o[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) {
-        const float f = fast_exp2(sm[w][rr] - base);
-        lsum = fmaf(f, sl[w][rr], lsum);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = fmaf(f, so[(w * 32 + rr) * ORS + 8 * ch + k], o[k]);
-      }
-      const int tk = (r0 + rr) / a.g;
-      const int64_t row = (s.lo + tk) * a.hq + h * a.g + (r0 + rr - tk * a.g);
-      if (a.npiece == 1) {
-        const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
-        E8 v;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (EL)(lsum != 0.f ? o[k] * inv : 0.f);
-        *reinterpret_cast<E8*>(a.out + row * D + 8 * ch) = v;
-      } else {
-        float* const pp = a.part + (row * a.npiece + pc) * (D + 2);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) pp[8 * ch + k] = o[k];
-        if (ch == 0) pp[D] = m, pp[D + 1] = lsum;
-      }
-    }
-    __syncthreads();
   }
 }
 
-// Joins the pieces of a row: one workgroup a (token, query head).
+// Joins the parts of a row of the sequence that the boundary behind stretch
+// blockIdx.x is the first to cut.
 template <typename EL, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
-  const int64_t row = blockIdx.x, n = row / a.hq;
-  const int tid = threadIdx.x, l = tid & 63;
-  const int b = paged_seq_of(a.c.cu, a.c.nseq, n);
-  if (b == a.c.nseq || n < a.c.cu[b]) {
-    if (a.zero_rest && tid < D / 8) reinterpret_cast<u32x4*>(a.out + row * D)[tid] = u32x4{};
-    return;
-  }
-  const PagedSeq s(a, b);
-  const int p = s.len - s.nq + (int)(n - s.lo);
-  const bool valid = p >= 0 && (a.sel == nullptr || a.sel[n] != 0);
-  // the pieces that hold keys which the row sees
-  const int lo = a.window >= 0 ? max(0, p - a.window) : 0;
-  const int p0 = min(lo / a.chunk, a.npiece - 1), p1 = valid ? min(p / a.chunk, a.npiece - 1) + 1 : p0;
-  constexpr int CH = D / 4, GR = 256 / CH;
-  const int ch = tid % CH, gr = tid / CH;
-  const float* const pp = a.part + row * a.npiece * (D + 2);
+__global__ __launch_bounds__(256) void paged_few_join_kernel(const PagedArgs a) {
+  const int w = blockIdx.x + 1, row = blockIdx.y, tid = threadIdx.x, l = tid & 63;
+  FewCut cut;
+  cut.init(a);
+  const int64_t at = w * cut.share;
+  if (at >= cut.total * a.c.heads) return;
+  int64_t rest;
+  const int h = cut.head_of(at, rest);
+  cut.locate(a, rest);
+  const int64_t f = rest - cut.start;
+  if (f == 0 || f > cut.share) return;
+  const PagedSeq s(a, cut.b);
+  const int rows = s.nq * a.g;
+  if (row >= rows || rows > a.part_rows) return;
+  const int np = 1 + (int)((cut.units - f + cut.share - 1) / cut.share);
+  constexpr int CL = D / 4, GR = 256 / CL;
+  const int ch = tid % CL, gr = tid / CL;
+  auto part = [&](int k) { return a.part + ((int64_t)(2 * (w - 1 + k) + (k == 0 ? 1 : 0)) * a.part_rows + row) * (D + 2); };
   __shared__ float red[4];
   __shared__ float so[GR][D + 4];
   float m = -INFINITY;
-  for (int k = p0 + tid; k < p1; k += 256) m = fmaxf(m, pp[(int64_t)k * (D + 2) + D]);
+  for (int k = tid; k < np; k += 256) m = fmaxf(m, part(k)[D]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
   if (l == 0) red[tid >> 6] = m;
@@ -250,12 +385,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   const float base = m == -INFINITY ? 0.f : m;
   f32x4 o = f32x4{};
   float ls = 0.f;
-  for (int k = p0 + gr; k < p1; k += GR) {
-    const float* const q = pp + (int64_t)k * (D + 2);
-    const float f = fast_exp2(q[D] - base);
-    ls = fmaf(f, q[D + 1], ls);
+#pragma unroll 4
+  for (int k = gr; k < np; k += GR) {
+    const float* const q = part(k);
+    const float x = fast_exp2(q[D] - base);
+    ls = fmaf(x, q[D + 1], ls);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(f, q[4 * ch + e], o[e]);
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(x, q[4 * ch + e], o[e]);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) so[gr][4 * ch + e] = o[e];
@@ -265,56 +401,51 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
     float v = 0.f, sum = 0.f;
 #pragma unroll
     for (int k = 0; k < GR; ++k) v += so[k][tid], sum += so[k][D];
-    reinterpret_cast<EL*>(a.out)[row * D + tid] = (EL)(sum != 0.f ? v / sum : 0.f);
+    const int tk = row / a.g;
+    reinterpret_cast<EL*>(a.out)[((s.lo + tk) * a.hq + h * a.g + row - tk * a.g) * D + tid] =
+        (EL)(sum != 0.f ? v / sum : 0.f);
   }
 }
 
-// Whether a call's rows go 32 at a time through the kernel for few rows: where no
-// sequence has more (by the caller's bound; others stay right, 32 after 32).
-static bool paged_few(int max_q, int g) { return (int64_t)max_q * g <= 32; }
-
-// How the keys are cut: pieces per sequence and keys per piece (a multiple of 128).
+// How a call runs: the kernel, whether and how finely keys may be cut, and the workspace.
 struct PagedPlan {
-  bool few;
-  int npiece, chunk;
+  bool few, split;
+  int target, cap, part_rows, nw;
   size_t part_bytes, bytes;
 };
 
 static PagedPlan paged_plan(int nseq, int h, int hq, int64_t n, int d, int max_q, int max_len, int window, bool sel) {
   PagedPlan p{};
-  const int g = hq / h;
-  p.few = paged_few(max_q, g);
-  max_len = std::max(max_len, 1);
-  int64_t want = 1;
-  if (window < 0) {  // a window's keys are few
-    const int64_t wgs = (p.few ? (int64_t)nseq : n * g / kTileRows + nseq) * h;
-    if (p.few) want = std::min<int64_t>((1024 + wgs - 1) / wgs, (max_len + 255) / 256);
-    else if (wgs < 384) want = std::min<int64_t>((1024 + wgs - 1) / wgs, (max_len + 511) / 512);
+  const int g = hq / h, cus = device_cus();
+  // up to 32 rows a sequence (by the caller's bound) share one pass of its keys
+  p.few = (int64_t)max_q * g <= 32;
+  const int64_t span = window >= 0 ? std::min<int64_t>(max_len, (int64_t)window + max_q) : max_len;
+  int64_t parts;
+  if (p.few) {
+    p.split = span > kFewUnit * kFewMinShare;
+    p.target = cus * (int)(160 * 1024 / (d == 128 ? few_smem<128>() : few_smem<64>()));
+    p.part_rows = std::max(1, max_q * g);
+    parts = 2 * p.target;
+  } else {
+    tile_plan(nseq, h, g, n, span, cus, sel, p.split, p.target, p.cap, p.nw);
+    p.part_rows = 32 * p.nw;
+    parts = (int64_t)p.cap * h;
   }
-  const int64_t per = (max_len + want - 1) / want;
-  p.chunk = (int)std::min<int64_t>((per + 127) & ~(int64_t)127, (int64_t)1 << 30);
-  p.npiece = (max_len + p.chunk - 1) / p.chunk;
-  if (p.npiece > 1) p.part_bytes = ((size_t)n * hq * p.npiece * (d + 2) * sizeof(float) + 255) & ~(size_t)255;
+  if (p.split) p.part_bytes = ((size_t)parts * p.part_rows * (d + 2) * sizeof(float) + 255) & ~(size_t)255;
   p.bytes = p.part_bytes + (sel && !p.few ? ((size_t)n + nseq) * sizeof(int32_t) : 0);
   return p;
 }
 
 template <typename EL, int D>
-static int paged_launch(const PagedArgs& a, bool few, int h, hipStream_t st) {
-  if (few) {
-    auto kern = paged_few_kernel<EL, D>;
-    LOGO_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<D>()));
-    const bool rest = a.npiece == 1 && a.zero_rest;
-    hipLaunchKernelGGL(kern, dim3(a.npiece, h, a.c.nseq + (rest ? 1 : 0)), dim3(64 * kFewWaves), few_smem<D>(), st, a);
-    LOGO_LAUNCH_CHECK("paged_few_kernel");
-  } else {
-    const int rc = paged_launch_tile(a, h, D, Elem<EL>::kHalf, st);
-    if (rc != LOGO_OK) return rc;
-  }
-  if (a.npiece > 1) {
-    hipLaunchKernelGGL((paged_join_kernel<EL, D>), dim3((unsigned)(a.n * a.hq)), dim3(256), 0, st, a);
-    LOGO_LAUNCH_CHECK("paged_join_kernel");
+static int few_launch(const PagedArgs& a, hipStream_t st) {
+  auto kern = paged_few_kernel<EL, D>;
+  LOGO_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)few_smem<D>()));
+  hipLaunchKernelGGL(kern, dim3(a.target), dim3(64 * kFewWaves), few_smem<D>(), st, a);
+  LOGO_LAUNCH_CHECK("paged_few_kernel");
+  if (a.split) {
+    hipLaunchKernelGGL((paged_few_join_kernel<EL, D>), dim3(a.target - 1, a.part_rows), dim3(256), 0, st, a);
+    LOGO_LAUNCH_CHECK("paged_few_join_kernel");
   }
   return LOGO_OK;
 }
@@ -325,7 +456,7 @@ using namespace logo;
 
 extern "C" size_t logo_paged_attn_workspace_bytes(int nseq, int h, int hq, int64_t n_tokens, int d, int max_q,
                                                   int max_len, int window, int selected) {
-  if (nseq < 1 || h < 1 || hq < h || n_tokens < 1) return 0;
+  if (nseq < 1 || h < 1 || hq < h || n_tokens < 1 || max_q < 0 || max_len < 0) return 0;
   return paged_plan(nseq, h, hq, n_tokens, d, max_q, max_len, window, selected != 0).bytes;
 }
 
@@ -360,16 +491,21 @@ extern "C" int logo_paged_attn(const logo_paged_cache* cache, const void* q, int
   a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.zero_rest = zero_rest != 0;
-  const PagedPlan plan = paged_plan(std::max(a.c.nseq, 1), h, hq, n_tokens, d, max_q, max_len, window, selection != nullptr);
-  LOGO_REQUIRE(a.c.nseq == 0 || plan.bytes == 0 || (workspace != nullptr && workspace_bytes >= plan.bytes),
-               "the workspace is too small");
-  a.npiece = a.c.nseq == 0 ? 1 : plan.npiece;
-  a.chunk = plan.chunk;
+  PagedPlan plan{};
+  plan.few = true;
+  plan.target = device_cus();
+  if (a.c.nseq > 0) plan = paged_plan(a.c.nseq, h, hq, n_tokens, d, max_q, max_len, window, selection != nullptr);
+  LOGO_REQUIRE(plan.bytes == 0 || (workspace != nullptr && workspace_bytes >= plan.bytes), "the workspace is too small");
+  a.split = plan.split;
+  a.target = plan.target;
+  a.cap = plan.cap;
+  a.part_rows = plan.part_rows;
   a.part = static_cast<float*>(workspace);
   a.idx = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + plan.part_bytes);
   a.count = a.idx + n_tokens;
-  const bool few = plan.few || a.c.nseq == 0;
   hipStream_t st = as_stream(stream);
-  if (dtype == LOGO_DTYPE_BF16) return d == 128 ? paged_launch<bf16, 128>(a, few, h, st) : paged_launch<bf16, 64>(a, few, h, st);
-  return d == 128 ? paged_launch<f16, 128>(a, few, h, st) : paged_launch<f16, 64>(a, few, h, st);
+  const bool half = dtype == LOGO_DTYPE_F16;
+  if (!plan.few) return paged_launch_tile(a, h, d, half, plan.nw, st);
+  if (half) return d == 128 ? few_launch<f16, 128>(a, st) : few_launch<f16, 64>(a, st);
+  return d == 128 ? few_launch<bf16, 128>(a, st) : few_launch<bf16, 64>(a, st);
 }

@@ -51,20 +51,57 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedAr
   if (tid == 0) a.count[b] = done;
 }
 
-// What a workgroup takes of the launch's (sequence, row tile, key piece) triples of
-// one kv head: the rank-th of them.  By a whole wave.
+// The cut of a launch's rows and keys.  Where the row tiles of all kv heads fill less
+// than three quarters of the workgroups that the device holds (a.target), each tile's
+// keys are cut into pieces, up to two rounds of workgroups in all, of equal size for all
+// sequences (the longest one's keys over their number).  Every workgroup works out the
+// same from cu, lens and the selected tokens' counts.
+constexpr int kMaxPieces = 16;
+constexpr int kTileMinChunk = 512;  // keys
+
 struct TileWork {
-  int b, tile, piece, rows;
-  __device__ __forceinline__ bool find(const PagedArgs& a, int64_t rank, int tile_rows) {
+  int b, tile, rows;   // sequence, row tile, the sequence's rows
+  int npiece, chunk;   // pieces a row tile, keys a piece
+  int piece;
+  __device__ __forceinline__ static int rows_of(const PagedArgs& a, int b, int& len) {
+    len = 0;
+    if (b >= a.c.nseq) return 0;
+    const PagedSeq s(a, b);
+    len = s.len;
+    return max(0, a.sel ? min(a.count[b], s.nq) : s.nq) * a.g;
+  }
+  // The rank-th (row tile, piece) of a kv head, the latest rows of a sequence first (they see the most keys); with
+  // pieces = false the rank-th row tile.  By a whole wave; false: none.
+  __device__ __forceinline__ bool find(const PagedArgs& a, int rank, int tile_rows, bool pieces) {
     const int lane = threadIdx.x & 63;
-    for (int c = 0; c < a.c.nseq; c += 64) {
-      int r = 0;
-      if (c + lane < a.c.nseq) {
-        const PagedSeq s(a, c + lane);
-        r = max(0, a.sel ? a.count[c + lane] : s.nq) * a.g;
+    int len, r = rows_of(a, lane, len), nt = (r + tile_rows - 1) / tile_rows;
+    npiece = 1;
+    chunk = 0x7fffffff;
+    if (a.split) {
+      int total = nt, longest = nt > 0 ? len : 0;
+      for (int c = 64; c < a.c.nseq; c += 64) {
+        int x;
+        const int k = (rows_of(a, c + lane, x) + tile_rows - 1) / tile_rows;
+        total += k;
+        if (k > 0) longest = max(longest, x);
       }
-      const int nt = (r + tile_rows - 1) / tile_rows * a.npiece;
-      int pre = nt;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) {
+        total += __shfl_xor(total, off);
+        longest = max(longest, __shfl_xor(longest, off));
+      }
+      total = uniform(total);
+      longest = uniform(longest);
+      const int wgs = max(1, total * a.c.heads);
+      if (4 * wgs < 3 * a.target && a.window < 0) {
+        npiece = max(1, min(min(2 * a.target / wgs, kMaxPieces), longest / kTileMinChunk));
+        if (npiece > 1) chunk = ((longest + npiece - 1) / npiece + 127) & ~127;
+      }
+    }
+    const int per = pieces ? npiece : 1;
+    for (int c = 0; c < a.c.nseq; c += 64) {
+      if (c > 0) r = rows_of(a, c + lane, len), nt = (r + tile_rows - 1) / tile_rows;
+      int pre = nt * per;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
         const int o = __shfl_up(pre, off);
@@ -73,15 +110,15 @@ struct TileWork {
       const unsigned long long past = __ballot(rank < pre);
       if (past != 0) {
         const int j = __builtin_ctzll(past);
-        const int tiles = __shfl(nt, j);
-        const int k = (int)rank - (__shfl(pre, j) - tiles);
+        const int tiles = __builtin_amdgcn_readlane(nt, j);
+        const int k = rank - (__builtin_amdgcn_readlane(pre, j) - tiles * per);
         b = c + j;
-        rows = __shfl(r, j);
-        piece = k % a.npiece;
-        tile = tiles / a.npiece - 1 - k / a.npiece;  // the latest rows, with the most keys, first
+        rows = __builtin_amdgcn_readlane(r, j);
+        piece = k % per;
+        tile = tiles - 1 - k / per;
         return true;
       }
-      rank -= __shfl(pre, 63);
+      rank -= __builtin_amdgcn_readlane(pre, 63);
     }
     return false;
   }
@@ -158,21 +195,22 @@ void paged_tile_kernel(const PagedArgs a) {
   int rank, h;
   xcd_remap(blockIdx.x, a.c.heads, rank, h);
 
-  // zero rows: tokens that are not selected and those of no sequence, a slice of them a workgroup
-  if (a.npiece == 1 && (a.sel != nullptr || a.zero_rest)) {
+  // zero rows: tokens that are not selected and those of no sequence, a slice of them a
+  // workgroup, D / 8 lanes a row
+  if (a.sel != nullptr || a.zero_rest) {
+    constexpr int CH = D / 8;
     const int slices = (int)(gridDim.x / a.c.heads), per = (int)((a.n + slices - 1) / slices);
     const int64_t n0 = (int64_t)rank * per, first = a.c.cu[0], end = a.c.cu[a.c.nseq];
-    const int per_row = a.g * D / 8, cnt = (int)max((int64_t)0, min((int64_t)per, a.n - n0));
-    // 16-byte chunks of the slice's rows, all lanes' tests in flight together
-    for (int64_t e = tid; e < (int64_t)cnt * per_row; e += 64 * NW) {
-      const int64_t n = n0 + e / per_row;
+    const int cnt = (int)max((int64_t)0, min((int64_t)per, a.n - n0)) * a.g;
+    for (int e = tid / CH; e < cnt; e += 64 * NW / CH) {
+      const int64_t n = n0 + e / a.g;
       const bool inside = n >= first && n < end;
       if (inside ? a.sel == nullptr || a.sel[n] != 0 : !a.zero_rest) continue;
-      st_nt(reinterpret_cast<u32x4*>(a.out + (n * a.hq + h * a.g) * D) + e % per_row, u32x4{});
+      st_nt(reinterpret_cast<u32x4*>(a.out + (n * a.hq + h * a.g + e % a.g) * D) + tid % CH, u32x4{});
     }
   }
   TileWork w;
-  if (!w.find(a, rank, ROWS)) return;
+  if (!w.find(a, rank, ROWS, true)) return;
   const PagedSeq s(a, w.b);
   const int r0 = w.tile * ROWS, pos0 = s.len - s.nq;
   // token in the sequence of row r
@@ -182,20 +220,30 @@ void paged_tile_kernel(const PagedArgs a) {
   const bool valid = wr + i <= rl, active = wr <= rl;
   const int tok = token(r), hrow = r % a.g;   // and its query head in the group
   const int p = valid ? pos0 + tok : -1;
-  const int pmin = pos0 + __builtin_amdgcn_readfirstlane(token(min(wr, rl)));
-  const int pmax = active ? pos0 + __builtin_amdgcn_readfirstlane(token(min(wr + 31, rl))) : -1;
-  int kv_lo, kv_hi;
-  paged_range(a, s.len, pos0 + __builtin_amdgcn_readfirstlane(token(r0)), pos0 + __builtin_amdgcn_readfirstlane(token(rl)),
-              w.piece, kv_lo, kv_hi);
-  kv_lo &= ~63;
-  if (a.npiece > 1 && kv_lo >= kv_hi) return;
-  const int W = a.window, nt = max(0, (kv_hi - kv_lo + 63) >> 6);
+  // held as lane values: with scalar branches around the pipelined bodies the register
+  // allocator spills hundreds of values between them
+  int pmin = pos0 + token(min(wr, rl)), pmax = active ? pos0 + token(min(wr + 31, rl)) : -1;
+  pin(pmin);
+  pin(pmax);
+  // the keys that the workgroup's rows see, of its piece
+  const int W = a.window;
+  int kv_lo = WINDOW ? max(0, pos0 + uniform(token(r0)) - W) & ~63 : 0;
+  int kv_hi = pos0 + uniform(token(rl)) + 1;
+  if (w.npiece > 1) {
+    kv_lo = w.piece * w.chunk;
+    if (w.piece < w.npiece - 1) kv_hi = min(kv_hi, kv_lo + w.chunk);
+    if (kv_lo >= kv_hi) return;
+  }
+  const int nt = max(0, (kv_hi - kv_lo + 63) >> 6);
 
   E8 qreg[DS];
   {
     const bf16* const qrow = a.q + (s.lo + tok) * a.q_token + (h * a.g + hrow) * a.q_head + 8 * g;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) qreg[ds] = valid ? *reinterpret_cast<const E8*>(qrow + 16 * ds) : E8{};
+    // they have arrived here: waited for inside the loop, they would drain its copies each time
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) pin(qreg[ds]);
   }
   f32x16 oacc[DT];
 #pragma unroll
@@ -377,9 +425,9 @@ void paged_tile_kernel(const PagedArgs a) {
     }
   }
   const float l_tot = pair_sum(l_run);
-  if (a.npiece > 1) {
+  if (w.npiece > 1) {
     if (valid) {
-      float* const pp = a.part + (((s.lo + tok) * a.hq + h * a.g + hrow) * a.npiece + w.piece) * (D + 2);
+      float* const pp = a.part + (((int64_t)h * a.cap + rank) * ROWS + 32 * wave + i) * (D + 2);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -411,6 +459,43 @@ void paged_tile_kernel(const PagedArgs a) {
   }
 }
 
+// Joins the pieces of eight rows of a row tile a workgroup.
+constexpr int kJoinRows = 8;
+template <typename EL, int D, int NW>
+__global__ __launch_bounds__(256) void paged_tile_join_kernel(const PagedArgs a) {
+  constexpr int ROWS = 32 * NW, LANES = 256 / kJoinRows, V = D / LANES;  // 4 or 2 columns a lane
+  typedef float fv __attribute__((ext_vector_type(V)));
+  typedef EL ev __attribute__((ext_vector_type(V)));
+  const int h = blockIdx.y;
+  TileWork w;
+  if (!w.find(a, blockIdx.x / (ROWS / kJoinRows), ROWS, false) || w.npiece == 1) return;
+  const PagedSeq s(a, w.b);
+  const int r = w.tile * ROWS + blockIdx.x % (ROWS / kJoinRows) * kJoinRows + threadIdx.x / LANES;
+  const int col = threadIdx.x % LANES * V;
+  if (r >= w.rows) return;
+  const int tok = a.sel ? a.idx[s.lo + r / a.g] : r / a.g, p = s.len - s.nq + tok;
+  // pieces that hold keys which the row sees
+  const int np = p < 0 ? 0 : min(p / w.chunk, w.npiece - 1) + 1;
+  const int64_t step = (int64_t)ROWS * (D + 2);
+  const float* const pp = a.part + ((int64_t)h * a.cap + (blockIdx.x / (ROWS / kJoinRows)) * w.npiece) * step +
+                          (r - w.tile * ROWS) * (D + 2);
+  float m = -INFINITY;
+  for (int k = 0; k < np; ++k) m = fmaxf(m, pp[k * step + D]);
+  const float base = m == -INFINITY ? 0.f : m;
+  fv o = fv{};
+  float sum = 0.f;
+  for (int k = 0; k < np; ++k) {
+    const float f = fast_exp2(pp[k * step + D] - base);
+    sum = fmaf(f, pp[k * step + D + 1], sum);
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = fmaf(f, pp[k * step + col + e], o[e]);
+  }
+  ev v;
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = (EL)(sum != 0.f ? o[e] / sum : 0.f);
+  *reinterpret_cast<ev*>(reinterpret_cast<EL*>(a.out) + ((s.lo + tok) * a.hq + h * a.g + r % a.g) * D + col) = v;
+}
+
 template <typename EL, int D, int NW>
 static int tile_launch(const PagedArgs& a, int h, hipStream_t st) {
   if (a.sel != nullptr) {
@@ -418,28 +503,44 @@ static int tile_launch(const PagedArgs& a, int h, hipStream_t st) {
     LOGO_LAUNCH_CHECK("paged_select_kernel");
   }
   // each sequence may end inside a tile
-  const int64_t tiles = a.n * a.g / (32 * NW) + a.c.nseq, blocks = tiles * a.npiece * h;
-  LOGO_REQUIRE(blocks < ((int64_t)1 << 31), "grid too large");
+  const int64_t tiles = a.n * a.g / (32 * NW) + a.c.nseq, ranks = std::max<int64_t>(tiles, a.split ? a.cap : 0);
+  LOGO_REQUIRE(ranks * h < ((int64_t)1 << 31), "grid too large");
   auto kern = a.window >= 0 ? paged_tile_kernel<EL, D, true, NW> : paged_tile_kernel<EL, D, false, NW>;
   LOGO_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)tile_smem<D>()));
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(64 * NW), tile_smem<D>(), st, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(ranks * h)), dim3(64 * NW), tile_smem<D>(), st, a);
   LOGO_LAUNCH_CHECK("paged_tile_kernel");
+  if (a.split) {
+    // only tiles that are cut: their pieces fit a.cap
+    const int64_t cut = std::min<int64_t>(tiles, a.cap / 2);
+    hipLaunchKernelGGL((paged_tile_join_kernel<EL, D, NW>), dim3((unsigned)(cut * (32 * NW / kJoinRows)), h), dim3(256), 0,
+                       st, a);
+    LOGO_LAUNCH_CHECK("paged_tile_join_kernel");
+  }
   return LOGO_OK;
 }
 
 template <typename EL, int D>
-static int tile_dispatch(const PagedArgs& a, int h, hipStream_t st) {
-#ifdef PAGED_NW8
-  return tile_launch<EL, D, 8>(a, h, st);
-#else
-  return tile_launch<EL, D, 4>(a, h, st);
-#endif
+static int tile_dispatch(const PagedArgs& a, int h, int nw, hipStream_t st) {
+  return nw == 8 ? tile_launch<EL, D, 8>(a, h, st) : tile_launch<EL, D, 4>(a, h, st);
 }
 
-int paged_launch_tile(const PagedArgs& a, int h, int d, bool half, hipStream_t st) {
-  if (half) return d == 128 ? tile_dispatch<f16, 128>(a, h, st) : tile_dispatch<f16, 64>(a, h, st);
-  return d == 128 ? tile_dispatch<bf16, 128>(a, h, st) : tile_dispatch<bf16, 64>(a, h, st);
+// Eight waves (256 rows share a tile's copies) where at least two rounds of such
+// workgroups are sure, one on a CU; four elsewhere, two on a CU.
+void tile_plan(int nseq, int h, int g, int64_t n, int64_t span, int cus, bool sel, bool& split, int& target, int& cap,
+               int& nw) {
+  const int64_t rows = n * g;
+  nw = !sel && rows / 256 * h >= 2 * cus ? 8 : 4;
+  target = cus * 8 / nw;
+  // the selected rows may be few of all, else the row tiles are known but for the sequences' ends
+  split = span >= 2 * kTileMinChunk && (sel || 4 * (rows / (32 * nw)) * h < 3 * (int64_t)target);
+  const int64_t tiles = rows / (32 * nw) + nseq;
+  cap = split ? (int)std::max<int64_t>(1, std::min<int64_t>(2 * target / h, tiles * kMaxPieces)) : 0;
+}
+
+int paged_launch_tile(const PagedArgs& a, int h, int d, bool half, int nw, hipStream_t st) {
+  if (half) return d == 128 ? tile_dispatch<f16, 128>(a, h, nw, st) : tile_dispatch<f16, 64>(a, h, nw, st);
+  return d == 128 ? tile_dispatch<bf16, 128>(a, h, nw, st) : tile_dispatch<bf16, 64>(a, h, nw, st);
 }
 
 }  // namespace logo

@@ -146,7 +146,7 @@ def _cache(**kw):
     (dict(page_size=24), "page_size"), (dict(page_size=8), "page_size"), (dict(heads=0), "head count"),
     (dict(k_slot=60), "multiples of 8"), (dict(v_slot=56), "hold a row"), (dict(k=264), "16-byte"), (dict(k=None), "null"),
     (dict(table_row=2), "counts"), (dict(nseq=-1), "counts"), (dict(lens=None), "null"),
-    (dict(table_width=1 << 27, table_row=1 << 27), "2\\^31"), (dict(k_slot=1 << 27), "2 GB"),
+    (dict(table_width=1 << 27, table_row=1 << 27), "2\\^30"), (dict(k_slot=1 << 27), "2 GB"),
 ])
 def test_c_entries_refuse_bad_caches(kw, msg):
     """Before any HIP call (pointers are placeholders)."""
