@@ -5,7 +5,6 @@ PyTorch fallback: if the library is missing, or a tensor is not on a ROCm GPU,
 the ops raise.
 """
 
-import contextlib
 import ctypes
 import os
 import re
@@ -163,14 +162,6 @@ def ptr(t):
 def stream_of(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
-
-def on_device(t: torch.Tensor):
-    """Context in which ``t``'s device is the current one (a launch goes to the
-    current device, whatever device its stream belongs to)."""
-    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-_SAME_DEVICE = contextlib.nullcontext()
 
 # Optional per-launch timing hook: called as hook(name, "start"|"end") around
 # every kernel launch of the ops (bench.py records HIP events through it).

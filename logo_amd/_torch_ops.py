@@ -88,6 +88,26 @@ def _register_fakes():
     def _(q, k_cache, v_cache, lens, gate, thres, max_len, scale):
         return torch.empty_like(q)
 
+    @fake("logo_hip::paged_attn")
+    def _(q, k_pages, v_pages, block_table, cu_seqlens, lens, selection, max_q, max_len, scale, window):
+        return q.new_empty(q.shape)
+
+    @fake("logo_hip::paged_attn_out")
+    def _(q, k_pages, v_pages, block_table, cu_seqlens, lens, selection, max_q, max_len, scale, window, out):
+        return None
+
+    @fake("logo_hip::paged_append")
+    def _(k, v, k_pages, v_pages, block_table, cu_seqlens, lens, q, turns, head_dim, rot_dim, interleaved, amplitude):
+        return k.new_empty(q.shape if q is not None else (0, 0, k.shape[2]))
+
+    @fake("logo_hip::rotary")
+    def _(xs, positions, turns, head_dim, rot_dim, interleaved, amplitude, inverse):
+        return [x.new_empty(x.shape) for x in xs]
+
+    @fake("logo_hip::rotary_")
+    def _(xs, positions, turns, head_dim, rot_dim, interleaved, amplitude):
+        return None
+
 
 def generic_kernels(d: int, dtype: torch.dtype) -> bool:
     """Whether head dim ``d`` and element type ``dtype`` run on the library's

@@ -91,12 +91,17 @@ struct PagedDma {
     }
   }
   // `rows` valid rows (none or less: zeros) from slot `slot` of page `page` (negative: zeros) on, to dst
+  // (NT: streaming loads, for rows that no other workgroup reads)
+  template <bool NT = false>
   __device__ __forceinline__ void issue(bf16* dst, int page, int slot, int rows) const {
     const bf16* p = base + (int64_t)max(page, 0) * page_stride + (int64_t)slot * slot_stride;
     const int bytes = rows > 0 && page >= 0 ? ((min(rows, ROWS) - 1) * slot_stride + D) * 2 : 0;
     const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(p), (short)0, bytes, kBufRsrcWord3);
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) buf_load_lds16(r, dst + RPB * b * D, o[b]);
+    for (int b = 0; b < BLOCKS; ++b) {
+      if constexpr (NT) buf_load_lds16_nt(r, dst + RPB * b * D, o[b]);
+      else buf_load_lds16(r, dst + RPB * b * D, o[b]);
+    }
   }
 };
 

@@ -44,10 +44,7 @@ namespace logo {
 // of its own in LDS (K(0) V(0) K(1) V(1) ...), without a barrier in the loop: a slot is
 // filled again as soon as its tile has been read, so most of a CU's 160 KB of LDS is in
 // flight at any time, which HBM's latency needs.
-#ifndef FEW_WAVES
-#define FEW_WAVES 2
-#endif
-constexpr int kFewWaves = FEW_WAVES;
+constexpr int kFewWaves = 2;
 constexpr int kFewUnit = 64;      // keys
 constexpr int kFewMinShare = 4;   // units: the shortest stretch, unless a sequence ends
 
@@ -56,61 +53,43 @@ constexpr int few_slots() { return D == 128 ? 5 : 10; }
 template <int D>
 constexpr size_t few_smem() { return (size_t)kFewWaves * few_slots<D>() * 32 * D * sizeof(bf16); }
 
-// The sequences laid end to end, and where a stretch lies.
+// The sequences laid end to end, kv head by kv head.
 struct FewCut {
-  int64_t total, share;  // units a kv head; units a workgroup
-  int units, lo, b;      // the located sequence: its units, its first key, its index
-  int64_t start;         // its first unit
-  int own_units, own_lo; // the lane's sequence of the first 64
+  int total, share;  // units a kv head; units a workgroup
+  int units, lo, b;  // the located sequence: its units, its first key, its index
+  int start;         // its first unit
+  int n, first, pre; // the lane's sequence of the last 64 looked at: units, first key, units up to its end
 
-  // Units of sequence b's keys that some row sees, from key lo on (at least one where it has new tokens).
-  __device__ __forceinline__ static int units_of(const PagedArgs& a, int b, int& lo) {
-    lo = 0;
-    if (b >= a.c.nseq) return 0;
-    const PagedSeq s(a, b);
-    if (s.nq == 0) return 0;
-    if (a.sel != nullptr) {
-      bool any = false;
-      for (int t = 0; t < s.nq && !any; ++t) any = a.sel[s.lo + t] != 0;
-      if (!any) return 1;
+  // Looks at sequences c .. c + 63, a lane each: the units of the keys that some row of
+  // theirs sees (at least one where there are new tokens).
+  __device__ __forceinline__ void look(const PagedArgs& a, int c) {
+    const int lane = threadIdx.x & 63, b = c + lane;
+    n = first = 0;
+    if (b < a.c.nseq) {
+      const PagedSeq s(a, b);
+      bool any = s.nq > 0;
+      if (a.sel != nullptr) {
+        any = false;
+        for (int t = 0; t < s.nq && !any; ++t) any = a.sel[s.lo + t] != 0;
+      }
+      if (a.window >= 0) first = max(0, s.len - s.nq - a.window) & ~(kFewUnit - 1);
+      n = any ? max(1, (s.len - first + kFewUnit - 1) / kFewUnit) : s.nq > 0;
     }
-    if (a.window >= 0) lo = max(0, s.len - s.nq - a.window) & ~(kFewUnit - 1);
-    return max(1, (s.len - lo + kFewUnit - 1) / kFewUnit);
-  }
-  __device__ __forceinline__ static int scan(int v) {
-    const int lane = threadIdx.x & 63;
+    pre = n;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(v, off);
-      if (lane >= off) v += o;
+      const int o = __shfl_up(pre, off);
+      if (lane >= off) pre += o;
     }
-    return v;
   }
-  __device__ __forceinline__ void init(const PagedArgs& a) {
-    const int lane = threadIdx.x & 63;
-    own_units = units_of(a, lane, own_lo);
-    total = __builtin_amdgcn_readlane(scan(own_units), 63);
-    for (int c = 64; c < a.c.nseq; c += 64) {
-      int x;
-      total += __builtin_amdgcn_readlane(scan(units_of(a, c + lane, x)), 63);
-    }
-    share = max((int64_t)kFewMinShare, (total * a.c.heads + a.target - 1) / a.target);
-  }
-  // kv head of unit pos, and the rest
-  __device__ __forceinline__ int head_of(int64_t pos, int64_t& rest) const {
-    const int h = pos >> 32 == 0 && total >> 32 == 0 ? (int)((uint32_t)pos / (uint32_t)total) : (int)(pos / total);
-    rest = pos - h * total;
-    return h;
-  }
-  // The sequence that holds unit `rest` (< total) of a kv head.  By a whole wave.
-  __device__ __forceinline__ void locate(const PagedArgs& a, int64_t rest) {
-    const int lane = threadIdx.x & 63;
-    int64_t base = 0;
-    int n = own_units, first = own_lo;
+  // One pass over the sequences, by a whole wave: the sum of their units (rest < 0), or
+  // the sequence that holds unit `rest` of a kv head (or is number `seq`).
+  __device__ __forceinline__ void pass(const PagedArgs& a, int rest, int seq = -1) {
+    int base = 0;
     for (int c = 0; c < a.c.nseq; c += 64) {
-      if (c > 0) n = units_of(a, c + lane, first);
-      const int pre = scan(n);
-      const unsigned long long past = __ballot(rest < base + pre);
+      if (rest < 0 || a.c.nseq > 64) look(a, c);
+      const int lane = threadIdx.x & 63;
+      const unsigned long long past = __ballot(rest >= 0 && (seq < 0 ? rest < base + pre : c + lane == seq));
       if (past != 0) {
         const int j = __builtin_ctzll(past);
         b = c + j;
@@ -121,6 +100,8 @@ struct FewCut {
       }
       base += __builtin_amdgcn_readlane(pre, 63);
     }
+    total = base;
+    share = max(kFewMinShare, (base * a.c.heads + a.target - 1) / a.target);
   }
 };
 
@@ -139,19 +120,14 @@ void paged_few_kernel(const PagedArgs a) {
   const int w = blockIdx.x;
   if (a.zero_rest) {
     // tokens of no sequence
-    const int64_t end = a.c.nseq > 0 ? max(0, a.c.cu[a.c.nseq]) : 0, begin = a.c.nseq > 0 ? a.c.cu[0] : 0;
-    const int row = a.hq * CH;
-    for (int64_t n = w; n < begin; n += gridDim.x)
-      for (int e = tid; e < row; e += 64 * NW) reinterpret_cast<u32x4*>(a.out + n * a.hq * D)[e] = u32x4{};
-    for (int64_t n = end + w; n < a.n; n += gridDim.x)
-      for (int e = tid; e < row; e += 64 * NW) reinterpret_cast<u32x4*>(a.out + n * a.hq * D)[e] = u32x4{};
+    const int begin = a.c.nseq > 0 ? a.c.cu[0] : 0, behind = a.c.nseq > 0 ? a.c.cu[a.c.nseq] : 0;
+    if (begin > 0 || behind < a.n)
+#pragma unroll 1
+      for (int64_t n = w; n < a.n; n += gridDim.x)
+        if (n < begin || n >= behind)
+#pragma unroll 1
+          for (int e = tid; e < a.hq * CH; e += 64 * NW) reinterpret_cast<u32x4*>(a.out + n * a.hq * D)[e] = u32x4{};
   }
-  FewCut cut;
-  cut.init(a);
-  int64_t pos = w * cut.share, rest = 0;
-  const int64_t end = min(pos + cut.share, cut.total * a.c.heads);
-  if (pos >= end) return;
-  int h = cut.head_of(pos, rest);
   TileReader<D, kSwz> rd;
   rd.init();
   bf16* const ring = reinterpret_cast<bf16*>(paged_smem) + wave * SLOTS * TILE;
@@ -160,11 +136,26 @@ void paged_few_kernel(const PagedArgs a) {
   float* const sl = sm + NW * 32;
   const float c = a.scale_log2;
 
-  for (int n; pos < end; pos += n, rest += n) {
-    if (rest == cut.total) ++h, rest = 0;
-    cut.locate(a, rest);
-    const int f = (int)(rest - cut.start);  // units of the sequence before this stretch
-    n = (int)min((int64_t)(cut.units - f), end - pos);
+  FewCut cut;
+  int pos = 0, end = 0, rest = -1, h = 0, n = 0;
+#pragma unroll 1
+  for (;; pos += n, rest += n) {
+    if (pos >= end && rest >= 0) return;
+    if (rest >= 0 && rest == cut.total) ++h, rest = 0;
+    cut.pass(a, rest);
+    if (rest < 0) {  // the first pass: the stretch
+      const int all = cut.total * a.c.heads;
+      // the last one may end before it starts
+      if ((int64_t)w * cut.share >= all) return;
+      pos = w * cut.share;
+      end = min(pos + cut.share, all);
+      h = (uint32_t)pos / (uint32_t)cut.total;
+      rest = pos - h * cut.total;
+      n = 0;
+      continue;
+    }
+    const int f = rest - cut.start;  // units of the sequence before this stretch
+    n = min(cut.units - f, end - pos);
     const int b = uniform(cut.b);
     const PagedSeq s(a, b);
     const int rows = s.nq * a.g, pos0 = s.len - s.nq;
@@ -194,7 +185,7 @@ void paged_few_kernel(const PagedArgs a) {
       f32x16 oacc[DT];
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
-      float m_run = -INFINITY, l_run = 0.f;
+      float m_run = -INFINITY, l_run = 0.f, base = 0.f;
       const int first = lo + 32 * wave;
       const int nt = __ballot(p >= 0) != 0 && first < hi ? (hi - first + 32 * NW - 1) / (32 * NW) : 0;
       int page[2];        // of the groups of the tile whose copies go out next
@@ -213,14 +204,19 @@ void paged_few_kernel(const PagedArgs a) {
           const bool has = page[u] >= 0 && page[u] < a.c.pages;
           const uint32_t bit = 1u << (2 * (t & 15) + u);
           held = has ? held | bit : held & ~bit;
-          d.issue(slot + 16 * u * D, has ? page[u] : -1, j & ((1 << a.shift) - 1), t < nt ? s.len - j : 0);
+          d.template issue<true>(slot + 16 * u * D, has ? page[u] : -1, j & ((1 << a.shift) - 1), t < nt ? s.len - j : 0);
         }
         if (is_v) look_up(t + 1);
       };
       if (nt > 0) {
         look_up(0);
-#pragma unroll
-        for (int k = 0; k < SLOTS; ++k) issue(k & 1 ? dv : dk, ring + k * TILE, k / 2, k & 1);
+        // as a loop: the launch's first instructions come from memory, one line after the other
+#pragma unroll 1
+        for (int k = 0; k < SLOTS / 2; ++k) {
+          issue(dk, ring + 2 * k * TILE, k, false);
+          issue(dv, ring + (2 * k + 1) * TILE, k, true);
+        }
+        if (SLOTS & 1) issue(dk, ring + (SLOTS - 1) * TILE, SLOTS / 2, false);
       }
       // q has arrived here: waited for inside the loop, it would drain the copies each time
 #pragma unroll
@@ -251,7 +247,8 @@ void paged_few_kernel(const PagedArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         float mx = -INFINITY;
         uint32_t seen = 0xffffu;
-        if (j0 + 31 > pmin || a.window >= 0 || has != 3 || !valid) {
+        // (rows that are not valid may see what they like: their results are dropped)
+        if (j0 + 31 > pmin || a.window >= 0 || has != 3) {
           seen = 0;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -262,22 +259,25 @@ void paged_few_kernel(const PagedArgs a) {
           }
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[e]);
-        const float m_new = fmaxf(m_run, pair_max(mx) * c);
-        const float base = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = fast_exp2(m_run - base);
-        m_run = m_new;
+        for (int e = 0; e < 16; e += 2) mx = max3_f32(mx, sc[e], sc[e + 1]);
+        // the reference maximum moves only when the row's grew by more than 2^8 (or on its first key)
+        const float mxs = pair_max(mx) * c;
+        if (__ballot(mxs - m_run > 8.f)) {
+          const float m_new = fmaxf(m_run, mxs);
+          base = m_new == -INFINITY ? 0.f : m_new;
+          const float alpha = fast_exp2(m_run - base);
+          m_run = m_new;
+          l_run *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
+        }
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           sc[e] = fast_exp2(fmaf(sc[e], c, -base));
           sum += sc[e];
         }
-        l_run = l_run * alpha + sum;
-        if (__ballot(alpha != 1.f)) {
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
-        }
+        l_run += sum;
         // rows that are not written (p = -1) need no care
         const bool edge = __ballot(p >= 0 && seen != 0xffffu) != 0;
         if (edge && !paged_tile_finite<EL, D, 2>(rd, vt)) {
@@ -299,7 +299,8 @@ void paged_few_kernel(const PagedArgs a) {
       }
       // join the waves
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      const float l_tot = pair_sum(l_run);
+      const float l_tot = valid ? pair_sum(l_run) : 0.f;
+      if (!valid) m_run = -INFINITY;
       __syncthreads();  // every wave is done with its slots
       {
         float* const orow = so + (wave * 32 + i) * ORS;
@@ -329,8 +330,9 @@ void paged_few_kernel(const PagedArgs a) {
         for (int wv = 0; wv < NW; ++wv) {
           const float x = fast_exp2(sm[wv * 32 + rr] - base);
           lsum = fmaf(x, sl[wv * 32 + rr], lsum);
+          if (sl[wv * 32 + rr] != 0.f)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] = fmaf(x, so[(wv * 32 + rr) * ORS + 8 * ch + k], o[k]);
+            for (int k = 0; k < 8; ++k) o[k] = fmaf(x, so[(wv * 32 + rr) * ORS + 8 * ch + k], o[k]);
         }
         if (whole) {
           const int tk = (r0 + rr) / a.g;
@@ -352,24 +354,36 @@ void paged_few_kernel(const PagedArgs a) {
   }
 }
 
-// Joins the parts of a row of the sequence that the boundary behind stretch
-// blockIdx.x is the first to cut.
+// Joins the parts of a row (blockIdx.y) of a sequence that is cut: blockIdx.x runs
+// over the sequences of all kv heads (by_seq), or, where these are more, over the
+// boundaries between the stretches, the first inside a sequence standing for it.
 template <typename EL, int D>
-__global__ __launch_bounds__(256) void paged_few_join_kernel(const PagedArgs a) {
-  const int w = blockIdx.x + 1, row = blockIdx.y, tid = threadIdx.x, l = tid & 63;
+__global__ __launch_bounds__(256) void paged_few_join_kernel(const PagedArgs a, const bool by_seq) {
+  const int row = blockIdx.y, tid = threadIdx.x, l = tid & 63;
+  int w = blockIdx.x + 1;  // the stretch in which the sequence's second part lies
   FewCut cut;
-  cut.init(a);
-  const int64_t at = w * cut.share;
-  if (at >= cut.total * a.c.heads) return;
-  int64_t rest;
-  const int h = cut.head_of(at, rest);
-  cut.locate(a, rest);
-  const int64_t f = rest - cut.start;
-  if (f == 0 || f > cut.share) return;
+  int h, f;  // f: units of its first part
+  cut.pass(a, -1);
+  if (cut.total == 0) return;
+  if (by_seq) {
+    h = blockIdx.x / a.c.nseq;
+    cut.pass(a, 0, blockIdx.x - h * a.c.nseq);
+    const int pos = h * cut.total + cut.start;
+    w = (uint32_t)pos / (uint32_t)cut.share + 1;
+    f = w * cut.share - pos;
+    if (f >= cut.units) return;
+  } else {
+    if ((int64_t)w * cut.share >= cut.total * a.c.heads) return;
+    h = (uint32_t)(w * cut.share) / (uint32_t)cut.total;
+    const int rest = w * cut.share - h * cut.total;
+    cut.pass(a, rest);
+    f = rest - cut.start;
+    if (f == 0 || f > cut.share) return;
+  }
   const PagedSeq s(a, cut.b);
   const int rows = s.nq * a.g;
   if (row >= rows || rows > a.part_rows) return;
-  const int np = 1 + (int)((cut.units - f + cut.share - 1) / cut.share);
+  const int np = 1 + (cut.units - f + cut.share - 1) / cut.share;
   constexpr int CL = D / 4, GR = 256 / CL;
   const int ch = tid % CL, gr = tid / CL;
   auto part = [&](int k) { return a.part + ((int64_t)(2 * (w - 1 + k) + (k == 0 ? 1 : 0)) * a.part_rows + row) * (D + 2); };
@@ -416,7 +430,7 @@ struct PagedPlan {
 
 static PagedPlan paged_plan(int nseq, int h, int hq, int64_t n, int d, int max_q, int max_len, int window, bool sel) {
   PagedPlan p{};
-  const int g = hq / h, cus = device_cus();
+  const int g = hq / h, cus = std::max(1, device_cus());
   // up to 32 rows a sequence (by the caller's bound) share one pass of its keys
   p.few = (int64_t)max_q * g <= 32;
   const int64_t span = window >= 0 ? std::min<int64_t>(max_len, (int64_t)window + max_q) : max_len;
@@ -444,7 +458,10 @@ static int few_launch(const PagedArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3(a.target), dim3(64 * kFewWaves), few_smem<D>(), st, a);
   LOGO_LAUNCH_CHECK("paged_few_kernel");
   if (a.split) {
-    hipLaunchKernelGGL((paged_few_join_kernel<EL, D>), dim3(a.target - 1, a.part_rows), dim3(256), 0, st, a);
+    const int64_t seqs = (int64_t)a.c.heads * a.c.nseq;
+    const bool by_seq = seqs < a.target;
+    hipLaunchKernelGGL((paged_few_join_kernel<EL, D>), dim3(by_seq ? (int)seqs : a.target, a.part_rows), dim3(256), 0, st,
+                       a, by_seq);
     LOGO_LAUNCH_CHECK("paged_few_join_kernel");
   }
   return LOGO_OK;
@@ -471,6 +488,8 @@ extern "C" int logo_paged_attn(const logo_paged_cache* cache, const void* q, int
   LOGO_REQUIRE(hq >= 1 && hq % h == 0, "query heads (%d) must be a multiple of the cache's heads (%d)", hq, h);
   LOGO_REQUIRE(cache->nseq <= 65534, "at most 65534 sequences");
   LOGO_REQUIRE(n_tokens >= 0 && n_tokens * hq < ((int64_t)1 << 31), "too many query rows");
+  LOGO_REQUIRE((int64_t)cache->nseq * ((int64_t)cache->table_width * cache->page_size / kFewUnit + 1) * h < ((int64_t)1 << 31),
+               "sequences x table x heads must stay below 2^31 units of %d keys", kFewUnit);
   LOGO_REQUIRE(max_q >= 0 && max_len >= 0 && window >= -1, "bad max_q, max_len or window");
   LOGO_REQUIRE(scale > 0.f && isfinite(scale), "scale must be positive and finite");
   LOGO_REQUIRE(q_token % 8 == 0 && q_head % 8 == 0 && ((uintptr_t)q | (uintptr_t)out) % 16 == 0,
@@ -493,7 +512,7 @@ extern "C" int logo_paged_attn(const logo_paged_cache* cache, const void* q, int
   a.zero_rest = zero_rest != 0;
   PagedPlan plan{};
   plan.few = true;
-  plan.target = device_cus();
+  plan.target = std::max(1, device_cus());
   if (a.c.nseq > 0) plan = paged_plan(a.c.nseq, h, hq, n_tokens, d, max_q, max_len, window, selection != nullptr);
   LOGO_REQUIRE(plan.bytes == 0 || (workspace != nullptr && workspace_bytes >= plan.bytes), "the workspace is too small");
   a.split = plan.split;

@@ -15,11 +15,10 @@ from typing import Optional
 
 import torch
 
-from .. import _lib
+from .. import _torch_ops
 
 __all__ = ["RotaryPlan", "rotary_plan", "rotary", "rotary_", "RotaryFunction"]
 
-_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
 MAX_HEAD_DIM = 512
 
 
@@ -86,60 +85,8 @@ def rotary_plan(head_dim: int, theta: float = 10000.0, rot_dim: Optional[int] = 
                       torch.tensor(turns, dtype=torch.int64).to(device=device))
 
 
-def batch_token_strides(x: torch.Tensor):
-    """(batch, token, head) strides of ``[T, H, D]`` or ``[B, T, H, D]`` rows, 0
-    where a size of one makes a stride meaningless."""
-    s = [st if n > 1 else 0 for st, n in zip(x.stride()[:-1], x.shape[:-1])]
-    return (0, *s) if len(s) == 2 else tuple(s)
-
-
-def _check(xs, positions, plan, what):
-    if not 1 <= len(xs) <= 4:
-        raise ValueError(f"{what} takes one to four tensors")
-    x0 = xs[0]
-    for x in xs:
-        if x.dim() < 3 or x.shape[:-2] != x0.shape[:-2] or x.shape[-1] != plan.head_dim or x.dtype != x0.dtype:
-            raise ValueError(f"{what} needs [..., T, H, D] tensors of one type and shape prefix, D = {plan.head_dim}")
-    if x0.dtype not in _DTYPES:
-        raise ValueError(f"{what} takes bf16, fp16 or fp32 tensors, got {x0.dtype}")
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what}: positions must be int32 or int64")
-    lead = x0.shape[:-2]
-    if positions.dim() > len(lead) or any(p != n and p != 1 for p, n in zip(positions.shape[::-1], lead[::-1])):
-        raise ValueError(f"{what}: positions {tuple(positions.shape)} do not match the tokens {tuple(lead)}")
-    _lib.require_gpu(*xs, positions, plan.turns)
-    if any(t.device != x0.device for t in (*xs, positions, plan.turns)):
-        raise ValueError(f"{what}: tensors on different devices")
-
-
-def _launch(xs, ys, positions, plan, inverse):
-    """``ys`` <- rotated ``xs``, all ``[T, H, D]`` or ``[B, T, H, D]`` with dense rows."""
-    x0 = xs[0]
-    lead = x0.shape[:-2]
-    pos = positions.expand(lead).contiguous()
-    rows = (_lib.Rows * len(xs))()
-    live = 0
-    for x, y in zip(xs, ys):
-        if x.numel() == 0:
-            continue
-        r = rows[live]
-        r.x, r.y, r.heads = x.data_ptr(), y.data_ptr(), x.shape[-2]
-        r.x_batch, r.x_token, r.x_head = batch_token_strides(x)
-        r.y_batch, r.y_token, r.y_head = batch_token_strides(y)
-        live += 1
-    if live == 0:
-        return
-    with _lib.on_device(x0):
-        _lib.launch("logo_rotary", _lib.lib().logo_rotary, rows, live, _lib.ptr(pos), 32 if pos.dtype == torch.int32
-                    else 64, pos.numel(), lead[-1], plan.head_dim, _lib.ptr(plan.turns), plan.rot_dim,
-                    int(plan.interleaved), plan.amplitude, int(inverse), _DTYPES[x0.dtype], _lib.stream_of(x0))
-
-
-def _rows4(x):
-    """``x [..., T, H, D]`` with dense rows and at most one batch axis (a copy where it has none)."""
-    if x.dim() > 4:
-        x = x.reshape(-1, *x.shape[-3:])
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+def _args(plan):
+    return plan.turns, plan.head_dim, plan.rot_dim, plan.interleaved, plan.amplitude
 
 
 class RotaryFunction(torch.autograd.Function):
@@ -151,12 +98,7 @@ class RotaryFunction(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
         ctx.plan, ctx.inverse = plan, inverse
-        ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-        pos = positions
-        if xs[0].dim() > 4:
-            pos = positions.expand(xs[0].shape[:-2]).reshape(-1, xs[0].shape[-3])
-        _launch([_rows4(x) for x in xs], [_rows4(y) for y in ys], pos, plan, inverse)
-        return tuple(ys)
+        return tuple(_torch_ops.timed("logo_rotary", _torch_ops.ops().rotary, xs, positions, *_args(plan), inverse))
 
     @staticmethod
     def backward(ctx, *gys):
@@ -174,24 +116,16 @@ def rotary(tensors, positions, plan: RotaryPlan):
     their tokens' ``positions`` (int32 or int64, broadcast to ``[..., T]``, of
     either sign); returns new contiguous tensors.  Differentiable."""
     xs = list(tensors)
-    _check(xs, positions, plan, "rotary")
-    return list(RotaryFunction.apply(positions, plan, False, *xs))
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        return list(RotaryFunction.apply(positions, plan, False, *xs))
+    return _torch_ops.timed("logo_rotary", _torch_ops.ops().rotary, xs, positions, *_args(plan), False)
 
 
 def rotary_(tensors, positions, plan: RotaryPlan):
     """``rotary`` in place, without gradients; returns the tensors.  At most one
     batch axis, dense rows, and no two rows in the same memory."""
     xs = list(tensors)
-    _check(xs, positions, plan, "rotary_")
-    for x in xs:
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise ValueError("rotary_ has no gradient; use rotary")
-        if x.dim() > 4 or (x.stride(-1) != 1 and x.shape[-1] > 1):
-            raise ValueError("rotary_ needs [T, H, D] or [B, T, H, D] tensors with dense rows")
-        extent = x.shape[-1]
-        for st, n in sorted((st, n) for st, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
-            if st < extent:
-                raise ValueError("rotary_: rows share memory")
-            extent = st * (n - 1) + extent
-    _launch(xs, xs, positions, plan, False)
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        raise ValueError("rotary_ has no gradient; use rotary")
+    _torch_ops.timed("logo_rotary", _torch_ops.ops().rotary_, xs, positions, *_args(plan))
     return xs

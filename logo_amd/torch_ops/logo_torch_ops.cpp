@@ -20,7 +20,11 @@
 //   epilogue_fwd  logo_epilogue_fwd   logo/layers/logo.py:180-181, :225-226, :256-258
 //   epilogue_bwd  logo_epilogue_bwd   the autograd of epilogue_fwd
 //   decode_attn   logo_decode_attn    logo/layers/logo.py:228-249
+//   paged_attn    logo_paged_attn     the same over a paged cache, and :183-209 for chunks over it
+//   paged_append  logo_paged_append   logo/cache.py:97-118, logo/layers/logo.py:132-150
+//   rotary        logo_rotary         logo/modules/rotary.py:58-106
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
@@ -28,7 +32,10 @@
 
 #include <algorithm>
 #include <cstdlib>
+#include <initializer_list>
+#include <limits>
 #include <mutex>
+#include <optional>
 #include <utility>
 #include <vector>
 
@@ -336,6 +343,260 @@ at::Tensor decode_attn(const at::Tensor& q, const at::Tensor& k_cache, const at:
   return out;
 }
 
+// The paged cache's operators and the rotary embedding check everything themselves
+// (ValueError for what they refuse), for tensors of any device, so that their Python
+// callers only fill in defaults.
+
+#define NEED(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
+
+// All tensors on one ROCm GPU.
+void on_gpu(const char* what, std::initializer_list<const at::Tensor*> ts) {
+  const at::Tensor* first = nullptr;
+  for (const at::Tensor* t : ts) {
+    if (t == nullptr) continue;
+    TORCH_CHECK(t->is_cuda(), "logo_amd ops run only on a ROCm GPU (got a tensor on ", t->device(),
+                "); there is no CPU fallback");
+    if (first == nullptr) first = t;
+    NEED(t->device() == first->device(), what, ": tensors on different devices");
+  }
+}
+const at::Tensor* optional_ptr(const std::optional<at::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
+
+int float_code(at::ScalarType t) {
+  return t == at::kBFloat16 ? LOGO_DTYPE_BF16 : t == at::kHalf ? LOGO_DTYPE_F16 : t == at::kFloat ? LOGO_DTYPE_F32 : -1;
+}
+
+// Stride of dimension d, 0 where its size makes it meaningless.
+int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// Shapes and types of a paged cache and a call's sequences.
+void check_cache(const char* what, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                 const at::Tensor& cu, const at::Tensor& lens) {
+  NEED(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes() && v_pages.scalar_type() == k_pages.scalar_type(), what,
+       ": k_pages and v_pages must be [P, H, page_size, D] of one shape and type");
+  const int code = float_code(k_pages.scalar_type());
+  NEED(code == LOGO_DTYPE_BF16 || code == LOGO_DTYPE_F16, what, " takes bf16 or fp16 pages, got ", k_pages.scalar_type());
+  NEED(table.dim() == 2 && cu.dim() == 1 && lens.dim() == 1, what,
+       ": block_table must be [S, M], cu_seqlens [S + 1], lens [S]");
+  for (const at::Tensor* t : {&table, &cu, &lens})
+    NEED(t->scalar_type() == at::kInt, what, ": block_table, cu_seqlens and lens must be int32");
+  const int64_t S = lens.size(0), page = k_pages.size(2), D = k_pages.size(3);
+  NEED(table.size(0) == S && cu.size(0) == S + 1, what, ": block_table and cu_seqlens do not match ", S, " sequences");
+  NEED(D == 64 || D == 128, what, ": head dim ", D, " unsupported (64 or 128)");
+  NEED(page >= 16 && page <= 65536 && (page & (page - 1)) == 0, what,
+       ": page_size must be a power of two in [16, 65536], got ", page);
+  for (const at::Tensor* t : {&k_pages, &v_pages})
+    NEED(t->stride(3) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0 &&
+             t->stride(2) >= D && aligned16(*t),
+         what, ": rows of the pages must be dense and 16-byte aligned");
+}
+
+logo_paged_cache cache_arg(const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                           const at::Tensor& cu, const at::Tensor& lens) {
+  logo_paged_cache c{};
+  c.k = k_pages.data_ptr();
+  c.v = v_pages.data_ptr();
+  c.k_page = k_pages.stride(0), c.k_head = k_pages.stride(1), c.k_slot = k_pages.stride(2);
+  c.v_page = v_pages.stride(0), c.v_head = v_pages.stride(1), c.v_slot = v_pages.stride(2);
+  c.pages = k_pages.size(0);
+  c.heads = (int32_t)k_pages.size(1);
+  c.page_size = (int32_t)k_pages.size(2);
+  c.table = static_cast<const int32_t*>(table.data_ptr());
+  c.table_width = (int32_t)table.size(1);
+  c.table_row = table.size(0) > 1 ? table.stride(0) : table.size(1);
+  c.cu = static_cast<const int32_t*>(cu.data_ptr());
+  c.lens = static_cast<const int32_t*>(lens.data_ptr());
+  c.nseq = (int32_t)lens.size(0);
+  return c;
+}
+
+at::Tensor dense_columns(const at::Tensor& t) { return t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t; }
+
+// x [N, H, D] with rows that 16-byte accesses reach (a copy where they do not).
+at::Tensor rows16(const at::Tensor& x) {
+  const bool fits = x.stride(2) == 1 && stride_of(x, 0) % 8 == 0 && stride_of(x, 1) % 8 == 0 && aligned16(x);
+  return fits ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+// out: written in place, its rows behind the last sequence left as they are; else a new
+// tensor with zeros there.
+at::Tensor paged_attn_impl(const at::Tensor& q_in, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                           const at::Tensor& table_in, const at::Tensor& cu_in, const at::Tensor& lens_in,
+                           const std::optional<at::Tensor>& selection, int64_t max_q, int64_t max_len, double scale,
+                           int64_t window, const std::optional<at::Tensor>& out_in) {
+  const char* what = "paged_attn";
+  check_cache(what, k_pages, v_pages, table_in, cu_in, lens_in);
+  NEED(q_in.dim() == 3 && q_in.scalar_type() == k_pages.scalar_type() && q_in.size(2) == k_pages.size(3), what,
+       ": q must be [N, HQ, D] of the pages' head dim and type");
+  const int64_t N = q_in.size(0), HQ = q_in.size(1), D = q_in.size(2), H = k_pages.size(1);
+  NEED(H > 0 && HQ % H == 0, what, ": ", HQ, " query heads are no multiple of the pages' ", H);
+  NEED(scale > 0 && scale < std::numeric_limits<float>::max(), what, ": scale must be positive and finite, got ", scale);
+  NEED(window >= -1, what, ": window must be None or >= 0, got ", window);
+  NEED(!selection.has_value() || (selection->scalar_type() == at::kBool && selection->dim() == 1 && selection->size(0) == N),
+       what, ": selection must be bool [N]");
+  NEED(!out_in.has_value() || (out_in->sizes() == q_in.sizes() && out_in->scalar_type() == q_in.scalar_type() &&
+                               out_in->is_contiguous() && aligned16(*out_in)),
+       what, ": out must be contiguous, of q's shape and type");
+  on_gpu(what, {&k_pages, &v_pages, &table_in, &cu_in, &lens_in, &q_in, optional_ptr(selection), optional_ptr(out_in)});
+  const c10::OptionalDeviceGuard guard(k_pages.device());
+  at::Tensor out = out_in.has_value() ? *out_in : at::empty({N, HQ, D}, q_in.options());
+  if (N == 0 || HQ == 0) return out;
+  const at::Tensor q = rows16(q_in), table = dense_columns(table_in), cu = cu_in.contiguous(), lens = lens_in.contiguous();
+  const at::Tensor sel = selection.has_value() ? selection->contiguous() : at::Tensor();
+  const logo_paged_cache c = cache_arg(k_pages, v_pages, table, cu, lens);
+  const int64_t reach = (int64_t)c.table_width * c.page_size;
+  const int mq = (int)(max_q < 0 ? N : std::min(max_q, N)), ml = (int)(max_len < 0 ? reach : std::min(max_len, reach));
+  const int w = (int)std::min<int64_t>(window, INT32_MAX);
+  const size_t bytes = logo_paged_attn_workspace_bytes(c.nseq, (int)H, (int)HQ, N, (int)D, mq, ml, w, sel.defined());
+  const at::Tensor ws = bytes > 0 ? at::empty({(int64_t)bytes}, q.options().dtype(at::kByte)) : at::Tensor();
+  ok(logo_paged_attn(&c, cptr(q), stride_of(q, 0), stride_of(q, 1), out.data_ptr(),
+                     sel.defined() ? static_cast<const uint8_t*>(sel.data_ptr()) : nullptr, (int)HQ, N, (int)D, mq, ml,
+                     (float)scale, w, !out_in.has_value(), ws.defined() ? ws.data_ptr() : nullptr, bytes,
+                     float_code(q.scalar_type()), sp()),
+     "logo_paged_attn");
+  return out;
+}
+at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                      const at::Tensor& cu, const at::Tensor& lens, const std::optional<at::Tensor>& selection,
+                      int64_t max_q, int64_t max_len, double scale, int64_t window) {
+  return paged_attn_impl(q, k_pages, v_pages, table, cu, lens, selection, max_q, max_len, scale, window, std::nullopt);
+}
+void paged_attn_out(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                    const at::Tensor& cu, const at::Tensor& lens, const std::optional<at::Tensor>& selection,
+                    int64_t max_q, int64_t max_len, double scale, int64_t window, const at::Tensor& out) {
+  paged_attn_impl(q, k_pages, v_pages, table, cu, lens, selection, max_q, max_len, scale, window, out);
+}
+
+// How heads are rotated: checks, and the turns' pointer.
+const uint64_t* check_plan(const char* what, int64_t D, const at::Tensor& turns, int64_t head_dim, int64_t rot) {
+  NEED(head_dim == D, what, ": the plan is for head dim ", head_dim, ", not ", D);
+  NEED(rot >= 0 && rot <= D && rot % 2 == 0 && turns.scalar_type() == at::kLong && turns.dim() == 1 &&
+           turns.size(0) == rot / 2 && turns.is_contiguous(),
+       what, ": the plan's turns must be int64 [rot_dim / 2]");
+  return static_cast<const uint64_t*>(turns.data_ptr());
+}
+
+// Rotated q [N, HQ, D] (an empty tensor without q); turns: none, keys are stored as they are.
+at::Tensor paged_append(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& k_pages,
+                        const at::Tensor& v_pages, const at::Tensor& table_in, const at::Tensor& cu_in,
+                        const at::Tensor& lens_in, const std::optional<at::Tensor>& q_in,
+                        const std::optional<at::Tensor>& turns, int64_t head_dim, int64_t rot, bool interleaved,
+                        double amplitude) {
+  const char* what = "paged_append";
+  check_cache(what, k_pages, v_pages, table_in, cu_in, lens_in);
+  NEED(k_in.dim() == 3 && v_in.sizes() == k_in.sizes() && k_in.scalar_type() == k_pages.scalar_type() &&
+           v_in.scalar_type() == k_in.scalar_type() && k_in.size(1) == k_pages.size(1) && k_in.size(2) == k_pages.size(3),
+       what, ": k and v must be [N, H, D] of the pages' heads, head dim and type");
+  const int64_t N = k_in.size(0), D = k_in.size(2);
+  NEED(!q_in.has_value() || (q_in->dim() == 3 && q_in->size(0) == N && q_in->size(2) == D &&
+                             q_in->scalar_type() == k_in.scalar_type()),
+       what, ": q must be [N, HQ, D] of k's type");
+  const uint64_t* tp = turns.has_value() ? check_plan(what, D, *turns, head_dim, rot) : nullptr;
+  on_gpu(what, {&k_pages, &v_pages, &table_in, &cu_in, &lens_in, &k_in, &v_in, optional_ptr(q_in), optional_ptr(turns)});
+  const c10::OptionalDeviceGuard guard(k_pages.device());
+  const int64_t HQ = q_in.has_value() ? q_in->size(1) : 0;
+  at::Tensor out = at::empty({q_in.has_value() ? N : 0, HQ, D}, k_in.options());
+  if (N == 0 || k_in.size(1) == 0) return out;
+  const at::Tensor k = rows16(k_in), v = rows16(v_in), q = HQ > 0 ? rows16(*q_in) : at::Tensor();
+  const at::Tensor table = dense_columns(table_in), cu = cu_in.contiguous(), lens = lens_in.contiguous();
+  if (lens.size(0) == 0) return out.zero_();
+  const logo_paged_cache c = cache_arg(k_pages, v_pages, table, cu, lens);
+  ok(logo_paged_append(&c, cptr(k), stride_of(k, 0), stride_of(k, 1), cptr(v), stride_of(v, 0), stride_of(v, 1),
+                       q.defined() ? cptr(q) : nullptr, q.defined() ? stride_of(q, 0) : 0,
+                       q.defined() ? stride_of(q, 1) : 0, q.defined() ? out.data_ptr() : nullptr, (int)HQ, N, (int)D, tp,
+                       tp != nullptr ? (int)rot : 0, interleaved, (float)amplitude, float_code(k.scalar_type()), sp()),
+     "logo_paged_append");
+  return out;
+}
+
+void check_rotary(const char* what, at::TensorList xs, const at::Tensor& pos, const at::Tensor& turns, int64_t head_dim,
+                  int64_t rot) {
+  NEED(xs.size() >= 1 && xs.size() <= 4, what, " takes one to four tensors");
+  const at::Tensor& x0 = xs[0];
+  for (const at::Tensor& x : xs) {
+    bool same = x.dim() >= 3 && x.dim() == x0.dim() && x.size(-1) == head_dim && x.scalar_type() == x0.scalar_type();
+    for (int64_t d = 0; same && d < x.dim() - 2; ++d) same = x.size(d) == x0.size(d);
+    NEED(same, what, " needs [..., T, H, D] tensors of one type and shape prefix, D = ", head_dim);
+  }
+  NEED(float_code(x0.scalar_type()) >= 0, what, " takes bf16, fp16 or fp32 tensors, got ", x0.scalar_type());
+  NEED(pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong, what, ": positions must be int32 or int64");
+  const int64_t lead = x0.dim() - 2;
+  bool fits = pos.dim() <= lead;
+  for (int64_t d = 1; fits && d <= pos.dim(); ++d) fits = pos.size(-d) == 1 || pos.size(-d) == x0.size(lead - d);
+  NEED(fits, what, ": positions ", pos.sizes(), " do not match the tokens ", x0.sizes().slice(0, lead));
+  check_plan(what, head_dim, turns, head_dim, rot);
+  for (const at::Tensor& x : xs) on_gpu(what, {&x, &pos, &turns, &x0});
+}
+
+// x [..., T, H, D] with dense rows and at most one batch dimension (a copy where it has none).
+at::Tensor rows4(const at::Tensor& x) {
+  const at::Tensor y = x.dim() > 4 ? x.reshape({-1, x.size(-3), x.size(-2), x.size(-1)}) : x;
+  return y.size(-1) > 1 && y.stride(-1) != 1 ? y.contiguous() : y;
+}
+
+void launch_rotary(const std::vector<at::Tensor>& xs, const std::vector<at::Tensor>& ys, at::IntArrayRef lead,
+                   const at::Tensor& positions, const at::Tensor& turns, int64_t rot, bool interleaved, double amplitude,
+                   bool inverse) {
+  logo_rows rows[4] = {};
+  int live = 0;
+  for (size_t i = 0; i < xs.size(); ++i) {
+    const at::Tensor &x = xs[i], &y = ys[i];
+    if (x.numel() == 0) continue;
+    logo_rows& r = rows[live++];
+    const bool batch = x.dim() == 4;
+    r.x = x.data_ptr();
+    r.y = y.data_ptr();
+    r.x_batch = batch ? stride_of(x, 0) : 0, r.y_batch = batch ? stride_of(y, 0) : 0;
+    r.x_token = stride_of(x, -3), r.y_token = stride_of(y, -3);
+    r.x_head = stride_of(x, -2), r.y_head = stride_of(y, -2);
+    r.heads = (int32_t)x.size(-2);
+  }
+  if (live == 0) return;
+  const at::Tensor pos = positions.expand(lead).contiguous();
+  ok(logo_rotary(rows, live, cptr(pos), pos.scalar_type() == at::kInt ? 32 : 64, pos.numel(), lead.back(),
+                 (int)xs[0].size(-1), static_cast<const uint64_t*>(turns.data_ptr()), (int)rot, interleaved,
+                 (float)amplitude, inverse, float_code(xs[0].scalar_type()), sp()),
+     "logo_rotary");
+}
+
+std::vector<at::Tensor> rotary(at::TensorList xs, const at::Tensor& positions, const at::Tensor& turns, int64_t head_dim,
+                               int64_t rot, bool interleaved, double amplitude, bool inverse) {
+  check_rotary("rotary", xs, positions, turns, head_dim, rot);
+  const c10::OptionalDeviceGuard guard(positions.device());
+  std::vector<at::Tensor> in, out, flat;
+  for (const at::Tensor& x : xs) {
+    in.push_back(rows4(x));
+    out.push_back(at::empty(x.sizes(), x.options()));
+    flat.push_back(rows4(out.back()));
+  }
+  launch_rotary(in, flat, xs[0].sizes().slice(0, xs[0].dim() - 2), positions, turns, rot, interleaved, amplitude, inverse);
+  return out;
+}
+
+void rotary_(at::TensorList xs, const at::Tensor& positions, const at::Tensor& turns, int64_t head_dim, int64_t rot,
+             bool interleaved, double amplitude) {
+  check_rotary("rotary_", xs, positions, turns, head_dim, rot);
+  std::vector<at::Tensor> rows;
+  for (const at::Tensor& x : xs) {
+    NEED(x.dim() <= 4 && (x.size(-1) <= 1 || x.stride(-1) == 1), "rotary_ needs [T, H, D] or [B, T, H, D] tensors with dense rows");
+    // from the smallest stride up, each dimension must step over what the ones before it span
+    std::vector<std::pair<int64_t, int64_t>> dims;
+    for (int64_t d = 0; d < x.dim() - 1; ++d)
+      if (x.size(d) > 1) dims.emplace_back(x.stride(d), x.size(d));
+    std::sort(dims.begin(), dims.end());
+    int64_t extent = x.size(-1);
+    for (const auto& [st, n] : dims) {
+      NEED(st >= extent, "rotary_: rows share memory");
+      extent += st * (n - 1);
+    }
+    rows.push_back(x);
+  }
+  const c10::OptionalDeviceGuard guard(positions.device());
+  launch_rotary(rows, rows, xs[0].sizes().slice(0, xs[0].dim() - 2), positions, turns, rot, interleaved, amplitude, false);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(logo_hip, m) {
@@ -361,6 +622,26 @@ TORCH_LIBRARY(logo_hip, m) {
         "float eps) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("decode_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor lens, Tensor? gate, Tensor? thres, "
         "int max_len, float scale) -> Tensor");
+  m.def("paged_attn(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cu_seqlens, Tensor lens, "
+        "Tensor? selection, int max_q, int max_len, float scale, int window) -> Tensor");
+  m.def("paged_attn_out(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cu_seqlens, Tensor lens, "
+        "Tensor? selection, int max_q, int max_len, float scale, int window, Tensor(a!) out) -> ()");
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor block_table, "
+        "Tensor cu_seqlens, Tensor lens, Tensor? q, Tensor? turns, int head_dim, int rot_dim, bool interleaved, "
+        "float amplitude) -> Tensor");
+  m.def("rotary(Tensor[] xs, Tensor positions, Tensor turns, int head_dim, int rot_dim, bool interleaved, "
+        "float amplitude, bool inverse) -> Tensor[]");
+  m.def("rotary_(Tensor(a!)[] xs, Tensor positions, Tensor turns, int head_dim, int rot_dim, bool interleaved, "
+        "float amplitude) -> ()");
+}
+
+// These refuse tensors of other devices themselves.
+TORCH_LIBRARY_IMPL(logo_hip, CompositeExplicitAutograd, m) {
+  m.impl("paged_attn", &paged_attn);
+  m.impl("paged_attn_out", &paged_attn_out);
+  m.impl("paged_append", &paged_append);
+  m.impl("rotary", &rotary);
+  m.impl("rotary_", &rotary_);
 }
 
 TORCH_LIBRARY_IMPL(logo_hip, CUDA, m) {
