@@ -17,7 +17,9 @@
 //
 // Bound by memory: each row is read and written once.  A workgroup takes a few
 // tokens of one tensor; cos and sin of its tokens are worked out once into LDS
-// and serve all heads.
+// and serve all heads.  A thread keeps its place in the row and walks the rows, four
+// at a time in flight; the first four are on their way before the tokens' positions
+// are known.
 #include <math.h>
 
 #include <algorithm>
@@ -31,6 +33,7 @@ namespace logo {
 constexpr int kRotThreads = 256;
 constexpr int kRotMaxTok = 16;     // tokens per workgroup
 constexpr int kRotItems = 1024;    // items (row chunks) a workgroup aims for
+constexpr int kRotFlight = 4;      // items of a thread in flight
 constexpr int kRotMaxDim = 512;
 
 struct RotRows {
@@ -40,7 +43,7 @@ struct RotRows {
   int64_t y_batch, y_token, y_head;  // (paged rows: page, slot, head)
   int heads;
   int tok, hc;                       // tokens and heads per workgroup
-  uint32_t hc_magic;                 // ceil(2^32 / hc)
+  int hp, tp;                        // heads and tokens that its threads cover at once
   bool rotate, paged;
 };
 
@@ -48,11 +51,10 @@ struct RotArgs {
   RotRows r[4];
   const void* positions;  // int32 or int64 [n] (rotary), else null
   bool pos64;
-  int64_t n, per_batch;   // tokens; tokens per batch entry
+  uint32_t n, per_batch;  // tokens (below 2^31); tokens per batch entry
   const uint64_t* turns;  // [rot / 2]
   float amp;
   int rot, d, units, pair_units;  // units: items per row, of which pair_units rotate
-  uint32_t units_magic;
   bool inter, inverse;
   // append
   const int32_t* table;
@@ -89,106 +91,133 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t frac) {
 // What a workgroup knows of each of its tokens.
 struct RotTok {
   int64_t pos;    // position
-  int64_t x_off;  // batch and token part of the source row's offset
-  int64_t y_off;  // of the destination row's; paged: of the page and slot
+  int64_t y_off;  // batch and token part of the destination row's offset; paged: of the page and slot
   int state;      // 0: written; 1: zero row (no position); 2: nothing to write
 };
 
-template <typename T, int VEC, bool APPEND>
+template <typename T, int VEC, bool APPEND, bool INTER>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(const RotArgs a) {
   typedef T vec __attribute__((ext_vector_type(VEC)));
   const RotRows& r = a.r[blockIdx.z];
-  const int64_t n0 = (int64_t)blockIdx.x * r.tok;
+  const uint32_t n0 = blockIdx.x * (uint32_t)r.tok;
   const int h0 = blockIdx.y * r.hc;
   if (n0 >= a.n || h0 >= r.heads) return;
-  const int ntok = (int)min((int64_t)r.tok, a.n - n0), tid = threadIdx.x;
+  const int ntok = min(r.tok, (int)(a.n - n0)), tid = threadIdx.x;
   extern __shared__ __attribute__((aligned(16))) char rot_smem[];
   RotTok* const info = reinterpret_cast<RotTok*>(rot_smem);                      // [kRotMaxTok]
   float2* const cs = reinterpret_cast<float2*>(rot_smem + kRotMaxTok * sizeof(RotTok));  // [ntok][rot / 2]
+  // the thread's place: item u of rows (t0 + k tp, h0 + ht + j hp)
+  const int rg = tid / a.units, u = tid - rg * a.units, t0 = rg / r.hp, ht = rg - t0 * r.hp;
+  const int nh = min(r.hc, r.heads - h0), half = a.rot >> 1;
+  const bool works = t0 < r.tp, pair = u < a.pair_units;
+  const int e0 = !pair ? a.rot + VEC * (u - a.pair_units) : INTER ? 2 * VEC * u : VEC * u;
+  const int e1 = !pair ? e0 : INTER ? e0 + VEC : half + VEC * u;
+  const T* const x = static_cast<const T*>(r.x) + (int64_t)(h0 + ht) * r.x_head;
+  T* const y = static_cast<T*>(r.y) + (int64_t)(h0 + ht) * r.y_head;
+  // items in the order (token step, head step); four of them at a time
+  const int nj = (nh - ht + r.hp - 1) / r.hp, nk = (ntok - t0 + r.tp - 1) / r.tp;
+  const int items = works && ht < nh && nk > 0 ? nk * nj : 0;
+  vec v0[kRotFlight], v1[kRotFlight];
+  int ik = 0, ij = 0;  // the next item to load
+  auto load = [&](int q) {
+    const uint32_t n = n0 + t0 + ik * r.tp;
+    int64_t off = n * r.x_token;
+    if (!APPEND && a.per_batch < a.n) {
+      const uint32_t b = n / a.per_batch;
+      off = b * r.x_batch + (n - b * a.per_batch) * r.x_token;
+    }
+    const T* const xr = x + off + (int64_t)(ij * r.hp) * r.x_head;
+    v0[q] = ld_nt(reinterpret_cast<const vec*>(xr + e0));
+    if (pair) v1[q] = ld_nt(reinterpret_cast<const vec*>(xr + e1));
+    if (++ij == nj) ij = 0, ++ik;
+  };
+#pragma unroll
+  for (int q = 0; q < kRotFlight; ++q)
+    if (q < items) load(q);
+
+  // the frequency whose angles the thread works out (rot / 2 <= 256 = the threads), and of which tokens
+  const int steps = half > 0 ? kRotThreads / half : 1, my_t = half > 0 ? tid / half : 0, my_i = tid - my_t * half;
+  const uint64_t my_turns = r.rotate && my_t < steps && my_i < half ? a.turns[my_i] : 0;
   if constexpr (APPEND) {
-    for (int t = tid >> 6; t < ntok; t += kRotThreads / 64) {
-      const int64_t n = n0 + t;
-      const int b = paged_seq_of(a.cu, a.nseq, n);
-      RotTok k{0, n * r.x_token, n * r.y_token, 1};
-      if (b < a.nseq) {
-        const int lo = a.cu[b], hi = a.cu[b + 1];
-        k.pos = (int64_t)a.lens[b] - hi + n;
+    // the first wave, a lane a token
+    if (tid < 64) {
+      int cnt = 0;  // sequences that end at or before the lane's token
+      for (int c = 0; c < a.nseq; c += 64) {
+        const int32_t e = c + tid < a.nseq ? a.cu[c + tid + 1] : 0x7fffffff;
+        for (int t = 0; t < ntok; ++t) {
+          const int k = __builtin_popcountll(__ballot(e <= (int)n0 + t));
+          cnt += tid == t ? k : 0;
+        }
+      }
+      const int n = (int)n0 + tid;
+      RotTok k{0, n * r.y_token, 1};
+      if (tid < ntok && cnt < a.nseq) {
+        const int lo = a.cu[cnt], hi = a.cu[cnt + 1];
+        k.pos = (int64_t)a.lens[cnt] - hi + n;
         if (n >= lo && k.pos >= 0) k.state = 0;
       }
       if (r.paged) {
         const int64_t col = k.pos >> a.page_shift;
         int page = -1;
-        if (k.state == 0 && col < a.table_width) page = a.table[b * a.table_row + col];
+        if (k.state == 0 && col < a.table_width) page = a.table[cnt * a.table_row + col];
         const bool held = page >= 0 && page < a.pages;
         k.y_off = held ? page * r.y_batch + (k.pos & ((1 << a.page_shift) - 1)) * r.y_token : 0;
         if (!held) k.state = 2;
       }
-      if ((tid & 63) == 0) info[t] = k;
+      if (tid < ntok) info[tid] = k;
     }
   } else {
     if (tid < ntok) {
-      const int64_t n = n0 + tid, b = n / a.per_batch, t = n - b * a.per_batch;
+      const uint32_t n = n0 + tid, b = n / a.per_batch, t = n - b * a.per_batch;
       const int64_t p = a.pos64 ? static_cast<const int64_t*>(a.positions)[n] : static_cast<const int32_t*>(a.positions)[n];
-      info[tid] = RotTok{p, b * r.x_batch + t * r.x_token, b * r.y_batch + t * r.y_token, 0};
+      info[tid] = RotTok{p, b * r.y_batch + t * r.y_token, 0};
     }
   }
   __syncthreads();
-  const int half = a.rot >> 1;
   if (r.rotate) {
-    for (int t = 0; t < ntok; ++t)
-      for (int i = tid; i < half; i += kRotThreads) {
-        float2 v = turn_cos_sin((uint64_t)info[t].pos * a.turns[i]);
+    if (my_t < steps)
+      for (int t = my_t; t < ntok; t += steps) {
+        float2 v = turn_cos_sin((uint64_t)info[t].pos * my_turns);
         v.x *= a.amp;
         v.y *= a.inverse ? -a.amp : a.amp;
-        cs[t * half + i] = v;
+        cs[t * half + my_i] = v;
       }
     __syncthreads();
   }
-  const int nh = min(r.hc, r.heads - h0);
-  const int items = ntok * r.hc * a.units;
-  const T* const x = static_cast<const T*>(r.x);
-  T* const y = static_cast<T*>(r.y);
-  for (int idx = tid; idx < items; idx += kRotThreads) {
-    const int row = a.units == 1 ? idx : (int)__umulhi((uint32_t)idx, a.units_magic);
-    const int u = idx - row * a.units;
-    const int t = r.hc == 1 ? row : (int)__umulhi((uint32_t)row, r.hc_magic);
-    const int h = row - t * r.hc;
-    if (h >= nh) continue;
-    const RotTok k = info[t];
-    if (k.state == 2) continue;
-    const T* const xr = x + k.x_off + (int64_t)(h0 + h) * r.x_head;
-    T* const yr = y + k.y_off + (int64_t)(h0 + h) * r.y_head;
-    if (u < a.pair_units) {
-      const int e0 = a.inter ? 2 * VEC * u : VEC * u, e1 = a.inter ? e0 + VEC : half + VEC * u;
-      vec v0 = *reinterpret_cast<const vec*>(xr + e0), v1 = *reinterpret_cast<const vec*>(xr + e1);
-      if (r.rotate) {
+  int ok = 0, oj = 0;  // the next item to store
+  for (int it = 0; it < items; it += kRotFlight) {
+#pragma unroll
+    for (int q = 0; q < kRotFlight; ++q) {
+      if (it + q >= items) break;
+      const int t = t0 + ok * r.tp;
+      const RotTok k = info[t];
+      T* const yr = y + k.y_off + (int64_t)(oj * r.hp) * r.y_head;
+      if (++oj == nj) oj = 0, ++ok;
+      vec a0 = v0[q], a1 = v1[q];
+      if (it + q + kRotFlight < items) load(q);
+      if (pair && r.rotate) {
         const float2* const c = cs + t * half + VEC * u;
         T in[2 * VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) in[e] = v0[e], in[VEC + e] = v1[e];
+        for (int e = 0; e < VEC; ++e) in[e] = a0[e], in[VEC + e] = a1[e];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const int ia = a.inter ? 2 * e : e, ib = a.inter ? 2 * e + 1 : VEC + e;
-          const float p = (float)in[ia], q = (float)in[ib];
-          in[ia] = (T)(p * c[e].x - q * c[e].y);
-          in[ib] = (T)(q * c[e].x + p * c[e].y);
+          constexpr int S = INTER ? 2 : 1, B = INTER ? 1 : VEC;
+          const float p = (float)in[S * e], q2 = (float)in[S * e + B];
+          in[S * e] = (T)(p * c[e].x - q2 * c[e].y);
+          in[S * e + B] = (T)(q2 * c[e].x + p * c[e].y);
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v0[e] = in[e], v1[e] = in[VEC + e];
+        for (int e = 0; e < VEC; ++e) a0[e] = in[e], a1[e] = in[VEC + e];
       }
-      if (k.state == 1) v0 = vec{}, v1 = vec{};
-      *reinterpret_cast<vec*>(yr + e0) = v0;
-      *reinterpret_cast<vec*>(yr + e1) = v1;
-    } else {
-      const int e0 = a.rot + VEC * (u - a.pair_units);
-      vec v0 = *reinterpret_cast<const vec*>(xr + e0);
-      if (k.state == 1) v0 = vec{};
-      *reinterpret_cast<vec*>(yr + e0) = v0;
+      if (k.state == 1) a0 = vec{}, a1 = vec{};
+      if (k.state != 2) {
+        *reinterpret_cast<vec*>(yr + e0) = a0;
+        if (pair) *reinterpret_cast<vec*>(yr + e1) = a1;
+      }
     }
   }
 }
-
-static uint32_t magic_of(int d) { return (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); }
 
 // The widest vector of at most 16 bytes whose multiples all rows' offsets are.
 static int rot_vec(const RotArgs& a, int nr, int size) {
@@ -207,21 +236,23 @@ template <typename T, int VEC, bool APPEND>
 static int rot_launch(RotArgs a, int nr, bool inplace, hipStream_t st) {
   a.pair_units = a.rot / 2 / VEC;
   a.units = a.pair_units + (inplace ? 0 : (a.d - a.rot) / VEC);
-  a.units_magic = magic_of(a.units);
   int64_t gx = 1;
   int gy = 1, tok = 1;
   for (int i = 0; i < nr; ++i) {
     RotRows& r = a.r[i];
-    r.hc = std::min(r.heads, std::max(1, kRotItems / a.units));
-    r.hc_magic = magic_of(r.hc);
+    const int rows = std::max(1, kRotThreads / a.units);  // rows that the threads cover at once
+    r.hc = std::min(r.heads, std::max(rows, kRotItems / a.units));
+    r.hp = std::min(r.hc, rows);
+    r.tp = rows / r.hp;
     r.tok = std::max(1, std::min(kRotMaxTok, kRotItems / (r.hc * a.units)));
-    gx = std::max(gx, (a.n + r.tok - 1) / r.tok);
+    gx = std::max(gx, ((int64_t)a.n + r.tok - 1) / r.tok);
     gy = std::max(gy, (r.heads + r.hc - 1) / r.hc);
     tok = std::max(tok, r.tok);
   }
   LOGO_REQUIRE(gx < ((int64_t)1 << 31) && gy <= 65535, "too many tokens or heads");
   const size_t smem = kRotMaxTok * sizeof(RotTok) + (size_t)tok * (a.rot / 2) * sizeof(float2);
-  hipLaunchKernelGGL((rotary_kernel<T, VEC, APPEND>), dim3((unsigned)gx, gy, nr), dim3(kRotThreads), smem, st, a);
+  auto kern = a.inter ? rotary_kernel<T, VEC, APPEND, true> : rotary_kernel<T, VEC, APPEND, false>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)gx, gy, nr), dim3(kRotThreads), smem, st, a);
   LOGO_LAUNCH_CHECK("rotary_kernel");
   return LOGO_OK;
 }
@@ -257,7 +288,7 @@ extern "C" int logo_rotary(const logo_rows* rows, int n_rows, const void* positi
   if (rc != LOGO_OK) return rc;
   LOGO_REQUIRE(rows != nullptr && n_rows >= 1 && n_rows <= 4, "one to four tensors");
   LOGO_REQUIRE(position_bits == 32 || position_bits == 64, "positions must be int32 or int64");
-  LOGO_REQUIRE(n_tokens >= 0 && tokens_per_batch >= 1, "bad token counts");
+  LOGO_REQUIRE(n_tokens >= 0 && n_tokens < ((int64_t)1 << 31) && tokens_per_batch >= 1, "bad token counts");
   if (n_tokens == 0) return LOGO_OK;
   LOGO_REQUIRE(positions != nullptr, "null positions");
   RotArgs a{};
@@ -265,7 +296,7 @@ extern "C" int logo_rotary(const logo_rows* rows, int n_rows, const void* positi
   for (int i = 0; i < n_rows; ++i) {
     const logo_rows& s = rows[i];
     LOGO_REQUIRE(s.x && s.y && s.heads >= 1, "tensor %d: null pointer or no heads", i);
-    a.r[i] = RotRows{s.x, s.y, s.x_batch, s.x_token, s.x_head, s.y_batch, s.y_token, s.y_head, s.heads, 1, 1, 0, true,
+    a.r[i] = RotRows{s.x, s.y, s.x_batch, s.x_token, s.x_head, s.y_batch, s.y_token, s.y_head, s.heads, 1, 1, 1, 1, true,
                      false};
     // in place, what passes through stays where it is
     inplace = inplace && s.x == s.y && s.x_batch == s.y_batch && s.x_token == s.y_token && s.x_head == s.y_head;
@@ -273,8 +304,8 @@ extern "C" int logo_rotary(const logo_rows* rows, int n_rows, const void* positi
   if (inplace && rot == 0) return LOGO_OK;
   a.positions = positions;
   a.pos64 = position_bits == 64;
-  a.n = n_tokens;
-  a.per_batch = tokens_per_batch;
+  a.n = (uint32_t)n_tokens;
+  a.per_batch = (uint32_t)std::min(tokens_per_batch, n_tokens);
   a.turns = turns;
   a.amp = amplitude;
   a.rot = rot;
@@ -296,17 +327,16 @@ extern "C" int logo_paged_append(const logo_paged_cache* cache, const void* k, i
   if (rc != LOGO_OK) return rc;
   rc = paged_check(cache, d);
   if (rc != LOGO_OK) return rc;
-  LOGO_REQUIRE(n_tokens >= 0, "n_tokens must be >= 0");
+  LOGO_REQUIRE(n_tokens >= 0 && n_tokens < ((int64_t)1 << 31), "n_tokens must be in [0, 2^31)");
   LOGO_REQUIRE((q == nullptr) == (q_out == nullptr) && (q == nullptr || hq >= 1), "q needs an output and heads");
   if (n_tokens == 0 || cache->nseq == 0) return LOGO_OK;
   LOGO_REQUIRE(k && v, "null pointer argument");
   const logo_paged_cache& c = *cache;
   RotArgs a{};
-  a.r[0] = RotRows{k, c.k, 0, k_token, k_head, c.k_page, c.k_slot, c.k_head, c.heads, 1, 1, 0, rot > 0, true};
-  a.r[1] = RotRows{v, c.v, 0, v_token, v_head, c.v_page, c.v_slot, c.v_head, c.heads, 1, 1, 0, false, true};
-  a.r[2] = RotRows{q, q_out, 0, q_token, q_head, 0, (int64_t)hq * d, d, hq, 1, 1, 0, rot > 0, false};
-  a.n = n_tokens;
-  a.per_batch = n_tokens;
+  a.r[0] = RotRows{k, c.k, 0, k_token, k_head, c.k_page, c.k_slot, c.k_head, c.heads, 1, 1, 1, 1, rot > 0, true};
+  a.r[1] = RotRows{v, c.v, 0, v_token, v_head, c.v_page, c.v_slot, c.v_head, c.heads, 1, 1, 1, 1, false, true};
+  a.r[2] = RotRows{q, q_out, 0, q_token, q_head, 0, (int64_t)hq * d, d, hq, 1, 1, 1, 1, rot > 0, false};
+  a.n = a.per_batch = (uint32_t)n_tokens;
   a.turns = turns;
   a.amp = amplitude;
   a.rot = rot;

@@ -17,7 +17,7 @@ import torch
 
 from .. import _torch_ops
 
-__all__ = ["RotaryPlan", "rotary_plan", "rotary", "rotary_", "RotaryFunction"]
+__all__ = ["RotaryPlan", "rotary_plan", "rotary", "rotary_"]
 
 MAX_HEAD_DIM = 512
 
@@ -89,36 +89,12 @@ def _args(plan):
     return plan.turns, plan.head_dim, plan.rot_dim, plan.interleaved, plan.amplitude
 
 
-class RotaryFunction(torch.autograd.Function):
-    """``rotary`` as one autograd node: one launch forward, one (the transposed
-    rotation of the gradients that arrive) backward."""
-
-    @staticmethod
-    def forward(ctx, positions, plan, inverse, *xs):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions)
-        ctx.plan, ctx.inverse = plan, inverse
-        return tuple(_torch_ops.timed("logo_rotary", _torch_ops.ops().rotary, xs, positions, *_args(plan), inverse))
-
-    @staticmethod
-    def backward(ctx, *gys):
-        positions, = ctx.saved_tensors
-        live = [i for i, g in enumerate(gys) if g is not None]
-        gxs = [None] * len(gys)
-        if live:
-            for i, g in zip(live, RotaryFunction.apply(positions, ctx.plan, not ctx.inverse, *(gys[i] for i in live))):
-                gxs[i] = g
-        return (None, None, None, *gxs)
-
-
 def rotary(tensors, positions, plan: RotaryPlan):
     """Rotate ``[..., T, H_i, D]`` tensors (one to four of one shape prefix) by
     their tokens' ``positions`` (int32 or int64, broadcast to ``[..., T]``, of
-    either sign); returns new contiguous tensors.  Differentiable."""
-    xs = list(tensors)
-    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        return list(RotaryFunction.apply(positions, plan, False, *xs))
-    return _torch_ops.timed("logo_rotary", _torch_ops.ops().rotary, xs, positions, *_args(plan), False)
+    either sign); returns new contiguous tensors.  Differentiable: the backward
+    pass is one launch, the transposed rotation."""
+    return _torch_ops.timed("logo_rotary", _torch_ops.ops().rotary, list(tensors), positions, *_args(plan), False)
 
 
 def rotary_(tensors, positions, plan: RotaryPlan):

@@ -25,7 +25,9 @@
 //   rotary        logo_rotary         logo/modules/rotary.py:58-106
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <hip/hip_runtime_api.h>
@@ -575,6 +577,64 @@ std::vector<at::Tensor> rotary(at::TensorList xs, const at::Tensor& positions, c
   return out;
 }
 
+// The rotation with its gradient, the transposed rotation of the gradients that arrive
+// (by this operator again, so it has a gradient too).
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+variable_list call_rotary(at::TensorList xs, const at::Tensor& positions, const at::Tensor& turns, int64_t head_dim,
+                          int64_t rot, bool interleaved, double amplitude, bool inverse) {
+  static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("logo_hip::rotary", "").typed<std::vector<at::Tensor>(
+      at::TensorList, const at::Tensor&, const at::Tensor&, int64_t, int64_t, bool, double, bool)>();
+  return op.call(xs, positions, turns, head_dim, rot, interleaved, amplitude, inverse);
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  // (tensors inside a list would not be followed)
+  using Opt = std::optional<at::Tensor>;
+  static variable_list forward(AutogradContext* ctx, at::Tensor x0, Opt x1, Opt x2, Opt x3, at::Tensor positions,
+                               at::Tensor turns, int64_t head_dim, int64_t rot, bool interleaved, double amplitude,
+                               bool inverse) {
+    std::vector<at::Tensor> xs{x0};
+    for (const Opt& x : {x1, x2, x3})
+      if (x.has_value()) xs.push_back(*x);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions, turns});
+    ctx->saved_data["dims"] = std::vector<int64_t>{head_dim, rot, interleaved, inverse};
+    ctx->saved_data["amplitude"] = amplitude;
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_rotary(xs, positions, turns, head_dim, rot, interleaved, amplitude, inverse);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto d = ctx->saved_data["dims"].toIntVector();
+    std::vector<at::Tensor> live;
+    for (const at::Tensor& g : grads)
+      if (g.defined()) live.push_back(g);
+    if (!live.empty())
+      live = call_rotary(live, saved[0], saved[1], d[0], d[1], d[2] != 0, ctx->saved_data["amplitude"].toDouble(), d[3] == 0);
+    variable_list out;
+    size_t k = 0;
+    for (const at::Tensor& g : grads) out.push_back(g.defined() ? live[k++] : at::Tensor());
+    out.resize(11);  // absent tensors, positions, turns and the five numbers have none
+    return out;
+  }
+};
+
+std::vector<at::Tensor> rotary_autograd(at::TensorList xs, const at::Tensor& positions, const at::Tensor& turns,
+                                        int64_t head_dim, int64_t rot, bool interleaved, double amplitude, bool inverse) {
+  // without a gradient to give, as without autograd
+  bool need = false;
+  if (at::GradMode::is_enabled())
+    for (const at::Tensor& x : xs) need = need || x.requires_grad();
+  if (!need) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_rotary(xs, positions, turns, head_dim, rot, interleaved, amplitude, inverse);
+  }
+  NEED(xs.size() >= 1 && xs.size() <= 4, "rotary takes one to four tensors");
+  const auto x = [&](size_t i) { return i < xs.size() ? RotaryFunction::Opt(xs[i]) : std::nullopt; };
+  return RotaryFunction::apply(xs[0], x(1), x(2), x(3), positions, turns, head_dim, rot, interleaved, amplitude, inverse);
+}
+
 void rotary_(at::TensorList xs, const at::Tensor& positions, const at::Tensor& turns, int64_t head_dim, int64_t rot,
              bool interleaved, double amplitude) {
   check_rotary("rotary_", xs, positions, turns, head_dim, rot);
@@ -643,6 +703,8 @@ TORCH_LIBRARY_IMPL(logo_hip, CompositeExplicitAutograd, m) {
   m.impl("rotary", &rotary);
   m.impl("rotary_", &rotary_);
 }
+
+TORCH_LIBRARY_IMPL(logo_hip, Autograd, m) { m.impl("rotary", &rotary_autograd); }
 
 TORCH_LIBRARY_IMPL(logo_hip, CUDA, m) {
   m.impl("compact", &compact);
