@@ -527,7 +527,7 @@ typedef struct {
 } logo_rows;
 
 /*
- * Turns the first `rot` elements (even, <= d <= 512) of each row of up to four
+ * Turns the first `rot` elements (even, <= d <= 256) of each row of up to four
  * tensors by its token's position (int32 or int64 [n_tokens], position_bits 32 or
  * 64, of either sign): pairs (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved,
  *   a' = amplitude (a cos t - b sin t),  b' = amplitude (b cos t + a sin t),

@@ -17,8 +17,8 @@
 //
 // Bound by memory: each row is read and written once.  A workgroup takes a few
 // tokens of one tensor; cos and sin of its tokens are worked out once into LDS
-// and serve all heads.  A thread keeps its place in the row and walks the rows, four
-// at a time in flight; the first four are on their way before the tokens' positions
+// and serve all heads.  A thread keeps its place in the row and walks the rows, two
+// in flight at a time; the first two are on their way before the tokens' positions
 // are known.
 #include <math.h>
 
@@ -33,8 +33,8 @@ namespace logo {
 constexpr int kRotThreads = 256;
 constexpr int kRotMaxTok = 16;     // tokens per workgroup
 constexpr int kRotItems = 1024;    // items (row chunks) a workgroup aims for
-constexpr int kRotFlight = 4;      // items of a thread in flight
-constexpr int kRotMaxDim = 512;
+constexpr int kRotFlight = 2;      // items of a thread in flight
+constexpr int kRotMaxDim = 256;    // a row has at most as many items as a workgroup threads
 
 struct RotRows {
   const void* x;
@@ -43,7 +43,6 @@ struct RotRows {
   int64_t y_batch, y_token, y_head;  // (paged rows: page, slot, head)
   int heads;
   int tok, hc;                       // tokens and heads per workgroup
-  int hp, tp;                        // heads and tokens that its threads cover at once
   bool rotate, paged;
 };
 
@@ -55,6 +54,7 @@ struct RotArgs {
   const uint64_t* turns;  // [rot / 2]
   float amp;
   int rot, d, units, pair_units;  // units: items per row, of which pair_units rotate
+  int rows;                       // rows that the threads of a workgroup cover at once
   bool inter, inverse;
   // append
   const int32_t* table;
@@ -106,30 +106,35 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(const RotArgs a) {
   extern __shared__ __attribute__((aligned(16))) char rot_smem[];
   RotTok* const info = reinterpret_cast<RotTok*>(rot_smem);                      // [kRotMaxTok]
   float2* const cs = reinterpret_cast<float2*>(rot_smem + kRotMaxTok * sizeof(RotTok));  // [ntok][rot / 2]
-  // the thread's place: item u of rows (t0 + k tp, h0 + ht + j hp)
-  const int rg = tid / a.units, u = tid - rg * a.units, t0 = rg / r.hp, ht = rg - t0 * r.hp;
+  // the thread's place: item u of every a.rows-th (token, head) row from rg on
   const int nh = min(r.hc, r.heads - h0), half = a.rot >> 1;
-  const bool works = t0 < r.tp, pair = u < a.pair_units;
+  const int rg = tid / a.units, u = tid - rg * a.units;
+  const int dt = a.rows / nh, dh = a.rows - dt * nh;
+  const bool pair = u < a.pair_units;
   const int e0 = !pair ? a.rot + VEC * (u - a.pair_units) : INTER ? 2 * VEC * u : VEC * u;
   const int e1 = !pair ? e0 : INTER ? e0 + VEC : half + VEC * u;
-  const T* const x = static_cast<const T*>(r.x) + (int64_t)(h0 + ht) * r.x_head;
-  T* const y = static_cast<T*>(r.y) + (int64_t)(h0 + ht) * r.y_head;
-  // items in the order (token step, head step); four of them at a time
-  const int nj = (nh - ht + r.hp - 1) / r.hp, nk = (ntok - t0 + r.tp - 1) / r.tp;
-  const int items = works && ht < nh && nk > 0 ? nk * nj : 0;
+  const T* const x = static_cast<const T*>(r.x) + (int64_t)h0 * r.x_head;
+  T* const y = static_cast<T*>(r.y) + (int64_t)h0 * r.y_head;
+  const int items = rg < a.rows ? (ntok * nh - rg + a.rows - 1) / a.rows : 0;
   vec v0[kRotFlight], v1[kRotFlight];
-  int ik = 0, ij = 0;  // the next item to load
+  int it = rg / nh, ih = rg - it * nh;  // the next row to load
+  int ot = it, oh = ih;                 // and to store
+  auto next = [&](int& t, int& h) {
+    t += dt;
+    h += dh;
+    if (h >= nh) h -= nh, ++t;
+  };
   auto load = [&](int q) {
-    const uint32_t n = n0 + t0 + ik * r.tp;
+    const uint32_t n = n0 + it;
     int64_t off = n * r.x_token;
     if (!APPEND && a.per_batch < a.n) {
       const uint32_t b = n / a.per_batch;
       off = b * r.x_batch + (n - b * a.per_batch) * r.x_token;
     }
-    const T* const xr = x + off + (int64_t)(ij * r.hp) * r.x_head;
+    const T* const xr = x + off + (int64_t)ih * r.x_head;
     v0[q] = ld_nt(reinterpret_cast<const vec*>(xr + e0));
     if (pair) v1[q] = ld_nt(reinterpret_cast<const vec*>(xr + e1));
-    if (++ij == nj) ij = 0, ++ik;
+    next(it, ih);
   };
 #pragma unroll
   for (int q = 0; q < kRotFlight; ++q)
@@ -184,17 +189,16 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(const RotArgs a) {
       }
     __syncthreads();
   }
-  int ok = 0, oj = 0;  // the next item to store
-  for (int it = 0; it < items; it += kRotFlight) {
+  for (int k0 = 0; k0 < items; k0 += kRotFlight) {
 #pragma unroll
     for (int q = 0; q < kRotFlight; ++q) {
-      if (it + q >= items) break;
-      const int t = t0 + ok * r.tp;
+      if (k0 + q >= items) break;
+      const int t = ot;
       const RotTok k = info[t];
-      T* const yr = y + k.y_off + (int64_t)(oj * r.hp) * r.y_head;
-      if (++oj == nj) oj = 0, ++ok;
+      T* const yr = y + k.y_off + (int64_t)oh * r.y_head;
+      next(ot, oh);
       vec a0 = v0[q], a1 = v1[q];
-      if (it + q + kRotFlight < items) load(q);
+      if (k0 + q + kRotFlight < items) load(q);
       if (pair && r.rotate) {
         const float2* const c = cs + t * half + VEC * u;
         T in[2 * VEC];
@@ -236,14 +240,12 @@ template <typename T, int VEC, bool APPEND>
 static int rot_launch(RotArgs a, int nr, bool inplace, hipStream_t st) {
   a.pair_units = a.rot / 2 / VEC;
   a.units = a.pair_units + (inplace ? 0 : (a.d - a.rot) / VEC);
+  a.rows = std::max(1, kRotThreads / a.units);
   int64_t gx = 1;
   int gy = 1, tok = 1;
   for (int i = 0; i < nr; ++i) {
     RotRows& r = a.r[i];
-    const int rows = std::max(1, kRotThreads / a.units);  // rows that the threads cover at once
-    r.hc = std::min(r.heads, std::max(rows, kRotItems / a.units));
-    r.hp = std::min(r.hc, rows);
-    r.tp = rows / r.hp;
+    r.hc = std::min(r.heads, std::max(a.rows, kRotItems / a.units));
     r.tok = std::max(1, std::min(kRotMaxTok, kRotItems / (r.hc * a.units)));
     gx = std::max(gx, ((int64_t)a.n + r.tok - 1) / r.tok);
     gy = std::max(gy, (r.heads + r.hc - 1) / r.hc);
@@ -296,7 +298,7 @@ extern "C" int logo_rotary(const logo_rows* rows, int n_rows, const void* positi
   for (int i = 0; i < n_rows; ++i) {
     const logo_rows& s = rows[i];
     LOGO_REQUIRE(s.x && s.y && s.heads >= 1, "tensor %d: null pointer or no heads", i);
-    a.r[i] = RotRows{s.x, s.y, s.x_batch, s.x_token, s.x_head, s.y_batch, s.y_token, s.y_head, s.heads, 1, 1, 1, 1, true,
+    a.r[i] = RotRows{s.x, s.y, s.x_batch, s.x_token, s.x_head, s.y_batch, s.y_token, s.y_head, s.heads, 1, 1, true,
                      false};
     // in place, what passes through stays where it is
     inplace = inplace && s.x == s.y && s.x_batch == s.y_batch && s.x_token == s.y_token && s.x_head == s.y_head;
@@ -333,9 +335,9 @@ extern "C" int logo_paged_append(const logo_paged_cache* cache, const void* k, i
   LOGO_REQUIRE(k && v, "null pointer argument");
   const logo_paged_cache& c = *cache;
   RotArgs a{};
-  a.r[0] = RotRows{k, c.k, 0, k_token, k_head, c.k_page, c.k_slot, c.k_head, c.heads, 1, 1, 1, 1, rot > 0, true};
-  a.r[1] = RotRows{v, c.v, 0, v_token, v_head, c.v_page, c.v_slot, c.v_head, c.heads, 1, 1, 1, 1, false, true};
-  a.r[2] = RotRows{q, q_out, 0, q_token, q_head, 0, (int64_t)hq * d, d, hq, 1, 1, 1, 1, rot > 0, false};
+  a.r[0] = RotRows{k, c.k, 0, k_token, k_head, c.k_page, c.k_slot, c.k_head, c.heads, 1, 1, rot > 0, true};
+  a.r[1] = RotRows{v, c.v, 0, v_token, v_head, c.v_page, c.v_slot, c.v_head, c.heads, 1, 1, false, true};
+  a.r[2] = RotRows{q, q_out, 0, q_token, q_head, 0, (int64_t)hq * d, d, hq, 1, 1, rot > 0, false};
   a.n = a.per_batch = (uint32_t)n_tokens;
   a.turns = turns;
   a.amp = amplitude;

@@ -19,7 +19,7 @@ from .. import _torch_ops
 
 __all__ = ["RotaryPlan", "rotary_plan", "rotary", "rotary_"]
 
-MAX_HEAD_DIM = 512
+MAX_HEAD_DIM = 256
 
 
 @dataclass(frozen=True)

@@ -53,7 +53,7 @@ def test_rotary_and_gradients(gpu, dtype, kw):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("D,rot,inter", [(80, 80, False), (80, 20, True), (80, 20, False), (96, 48, True), (2, 2, False),
-                                         (6, 4, True), (100, 50, False), (512, 512, True), (256, 128, False), (1, 0, False)])
+                                         (6, 4, True), (100, 50, False), (256, 256, True), (256, 2, False), (256, 2, True), (256, 128, False), (1, 0, False)])
 def test_head_dims_and_parts(gpu, dtype, D, rot, inter):
     """Every vector width, odd halves and the scalar form; one token and three."""
     for T in (1, 3):

@@ -38,7 +38,7 @@ def test_plan_turns_wrap():
 
 
 @pytest.mark.parametrize("kw,msg", [
-    (dict(head_dim=0), "head_dim"), (dict(head_dim=513), "head_dim"), (dict(head_dim=64, rot_dim=66), "rot_dim"),
+    (dict(head_dim=0), "head_dim"), (dict(head_dim=257), "head_dim"), (dict(head_dim=64, rot_dim=66), "rot_dim"),
     (dict(head_dim=64, rot_dim=31), "rot_dim"), (dict(head_dim=64, rot_dim=-2), "rot_dim"), (dict(head_dim=63), "rot_dim"),
     (dict(head_dim=64, theta=0.0), "theta"), (dict(head_dim=64, theta=math.inf), "theta"),
     (dict(head_dim=64, scaling="dynamic"), "scaling"), (dict(head_dim=64, scaling="linear", factor=0.0), "factor"),
@@ -175,7 +175,7 @@ def test_c_entries_refuse_bad_arguments():
     rot = lambda n=1, bits=32, d=64, r=64, t=p, amp=1.0, dt=0: lib.logo_rotary(  # noqa: E731
         rows, n, p, bits, 5, 5, d, t, r, 0, amp, 0, dt, None)
     for kw, msg in ((dict(n=0), "one to four"), (dict(n=5), "one to four"), (dict(bits=16), "int32 or int64"),
-                    (dict(d=513), "head dim"), (dict(r=33), "even"), (dict(r=66), "even"), (dict(t=None), "turns"),
+                    (dict(d=257), "head dim"), (dict(r=33), "even"), (dict(r=66), "even"), (dict(t=None), "turns"),
                     (dict(amp=math.inf), "amplitude"), (dict(dt=5), "dtype"), (dict(), "null pointer")):
         assert rot(**kw) == 1 and msg in err(), kw
     assert lib.logo_paged_append(c, p, 128, 64, p, 128, 64, p, 256, 64, None, 4, 5, 64, None, 0, 0, 1.0, 0, None) == 1
