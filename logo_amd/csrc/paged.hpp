@@ -105,20 +105,15 @@ struct PagedDma {
   }
 };
 
-// Whether all values of `steps` 16-key steps of a V tile are finite: their products
-// with zero, which are NaN for the others, summed by the matrix unit.
-template <typename EL, int D, int STEPS>
-__device__ __forceinline__ bool paged_tile_finite(const TileReader<D, kSwz>& rd, const bf16* vt) {
-  using E8 = typename Elem<EL>::x8;
-  f32x16 z = f32x16{};
-#pragma unroll
-  for (int ks = 0; ks < STEPS; ++ks)
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) z = mfma32(rd.template tr<EL>(vt, 16 * ks, dt), E8{}, z);
+// Whether some element of a lane's outputs is NaN, for any lane whose row is valid.
+template <int DT>
+__device__ __forceinline__ bool paged_any_nan(const f32x16 (&oacc)[DT], bool valid) {
   float t = 0.f;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) t += z[e];
-  return __ballot(t != t) == 0;
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) t += oacc[dt][e] * 0.f;  // NaN for infinities too
+  return __ballot(valid && t != 0.f) != 0;
 }
 
 // O += V^T P over one 16-key step whose values may be infinite or NaN: those count

@@ -8,9 +8,10 @@
 // of page table[b, j / page_size].
 //
 // A key that a row does not see has weight zero, but zero times infinity or NaN is
-// NaN.  Where a tile crosses the edge of some row's keys, its values are therefore
-// tested, and if one is not finite they enter the product as zeros and only the
-// rows that see such a key get NaN (paged_tile_finite, paged_pv_guarded).
+// NaN, which stays in O.  So rows whose O is not finite at the end are worked out once
+// more, guarded: in tiles that cross the edge of some row's keys, values that are not
+// finite then count as zeros, and only the rows that see such a key get NaN
+// (paged_pv_guarded).
 //
 // Tiles.  A tile of keys is copied to LDS by buffer_load ... lds in groups of 16
 // keys: a page holds a multiple of 16, so a group's rows lie in one page and share
@@ -183,9 +184,7 @@ void paged_few_kernel(const PagedArgs a) {
         for (int ds = 0; ds < DS; ++ds) qreg[ds] = valid ? *reinterpret_cast<const E8*>(qrow + 16 * ds) : E8{};
       }
       f32x16 oacc[DT];
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
-      float m_run = -INFINITY, l_run = 0.f, base = 0.f;
+      float m_run, l_run, base;
       const int first = lo + 32 * wave;
       const int nt = __ballot(p >= 0) != 0 && first < hi ? (hi - first + 32 * NW - 1) / (32 * NW) : 0;
       int page[2];        // of the groups of the tile whose copies go out next
@@ -208,97 +207,104 @@ void paged_few_kernel(const PagedArgs a) {
         }
         if (is_v) look_up(t + 1);
       };
-      if (nt > 0) {
-        look_up(0);
-        // as a loop: the launch's first instructions come from memory, one line after the other
+      bool guard = false;
 #pragma unroll 1
-        for (int k = 0; k < SLOTS / 2; ++k) {
-          issue(dk, ring + 2 * k * TILE, k, false);
-          issue(dv, ring + (2 * k + 1) * TILE, k, true);
+      for (;;) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
+        m_run = -INFINITY, l_run = base = 0.f;
+        if (nt > 0) {
+          look_up(0);
+          // as a loop: the launch's first instructions come from memory, one line after the other
+#pragma unroll 1
+          for (int k = 0; k < SLOTS / 2; ++k) {
+            issue(dk, ring + 2 * k * TILE, k, false);
+            issue(dv, ring + (2 * k + 1) * TILE, k, true);
+          }
+          if (SLOTS & 1) issue(dk, ring + (SLOTS - 1) * TILE, SLOTS / 2, false);
         }
-        if (SLOTS & 1) issue(dk, ring + (SLOTS - 1) * TILE, SLOTS / 2, false);
-      }
-      // q has arrived here: waited for inside the loop, it would drain the copies each time
+        // q has arrived here: waited for inside the loop, it would drain the copies each time
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds) pin(qreg[ds]);
-      int at = 0;  // ring slot of the tile that is read next
-      for (int t = 0; t < nt; ++t) {
-        const int j0 = first + 32 * NW * t;
-        const uint32_t has = held >> (2 * (t & 15)) & 3;
-        const bf16* const kt = ring + at * TILE;
-        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(AHEAD) : "memory");
-        // all reads of the tile in flight at once; they are done before its slot's next copies
-        E8 op[2 * DT > DS ? 2 * DT : DS];
+        for (int ds = 0; ds < DS; ++ds) pin(qreg[ds]);
+        int at = 0;  // ring slot of the tile that is read next
+        for (int t = 0; t < nt; ++t) {
+          const int j0 = first + 32 * NW * t;
+          const uint32_t has = held >> (2 * (t & 15)) & 3;
+          const bf16* const kt = ring + at * TILE;
+          asm volatile("s_waitcnt vmcnt(%0)" ::"i"(AHEAD) : "memory");
+          // all reads of the tile in flight at once; they are done before its slot's next copies
+          E8 op[2 * DT > DS ? 2 * DT : DS];
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) op[ds] = rd.template row<EL>(kt, 0, ds);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        f32x16 sc = f32x16{};
+          for (int ds = 0; ds < DS; ++ds) op[ds] = rd.template row<EL>(kt, 0, ds);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_sched_barrier(0);
+          f32x16 sc = f32x16{};
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) sc = mfma32(op[ds], qreg[ds], sc);
-        // slot 2 t + SLOTS takes the place of K(t): a V where the ring is odd
-        issue(SLOTS & 1 ? dv : dk, ring + at * TILE, t + SLOTS / 2, SLOTS & 1);
-        at = at + 1 == SLOTS ? 0 : at + 1;
-        // V(t), read while S turns into P
-        const bf16* const vt = ring + at * TILE;
-        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(AHEAD) : "memory");
+          for (int ds = 0; ds < DS; ++ds) sc = mfma32(op[ds], qreg[ds], sc);
+          // slot 2 t + SLOTS takes the place of K(t): a V where the ring is odd
+          issue(SLOTS & 1 ? dv : dk, ring + at * TILE, t + SLOTS / 2, SLOTS & 1);
+          at = at + 1 == SLOTS ? 0 : at + 1;
+          // V(t), read while S turns into P
+          const bf16* const vt = ring + at * TILE;
+          asm volatile("s_waitcnt vmcnt(%0)" ::"i"(AHEAD) : "memory");
 #pragma unroll
-        for (int k = 0; k < 2 * DT; ++k) op[k] = rd.template tr<EL>(vt, 16 * (k / DT), k % DT);
-        __builtin_amdgcn_sched_barrier(0);
-        float mx = -INFINITY;
-        uint32_t seen = 0xffffu;
-        // (rows that are not valid may see what they like: their results are dropped)
-        if (j0 + 31 > pmin || a.window >= 0 || has != 3) {
-          seen = 0;
+          for (int k = 0; k < 2 * DT; ++k) op[k] = rd.template tr<EL>(vt, 16 * (k / DT), k % DT);
+          __builtin_amdgcn_sched_barrier(0);
+          float mx = -INFINITY;
+          uint32_t seen = 0xffffu;
+          // (rows that are not valid may see what they like: their results are dropped)
+          if (j0 + 31 > pmin || a.window >= 0 || has != 3) {
+            seen = 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int key = j0 + rowmap(g, e);
+              const bool vis = key <= p && (a.window < 0 || key >= p - a.window) && (has >> (e >> 3) & 1);
+              seen |= vis ? 1u << e : 0u;
+              sc[e] = vis ? sc[e] : -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) mx = max3_f32(mx, sc[e], sc[e + 1]);
+          // the reference maximum moves only when the row's grew by more than 2^8 (or on its first key)
+          const float mxs = pair_max(mx) * c;
+          if (__ballot(mxs - m_run > 8.f)) {
+            const float m_new = fmaxf(m_run, mxs);
+            base = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = fast_exp2(m_run - base);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
+          }
+          float sum = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int key = j0 + rowmap(g, e);
-            const bool vis = key <= p && (a.window < 0 || key >= p - a.window) && (has >> (e >> 3) & 1);
-            seen |= vis ? 1u << e : 0u;
-            sc[e] = vis ? sc[e] : -INFINITY;
+            sc[e] = fast_exp2(fmaf(sc[e], c, -base));
+            sum += sc[e];
           }
-        }
+          l_run += sum;
+          if (guard && __ballot(p >= 0 && seen != 0xffffu) != 0) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) mx = max3_f32(mx, sc[e], sc[e + 1]);
-        // the reference maximum moves only when the row's grew by more than 2^8 (or on its first key)
-        const float mxs = pair_max(mx) * c;
-        if (__ballot(mxs - m_run > 8.f)) {
-          const float m_new = fmaxf(m_run, mxs);
-          base = m_new == -INFINITY ? 0.f : m_new;
-          const float alpha = fast_exp2(m_run - base);
-          m_run = m_new;
-          l_run *= alpha;
+            for (int ks = 0; ks < 2; ++ks)
+              paged_pv_guarded<EL, D>(oacc, rd, vt, ks, acc_to<EL>(sc, ks), seen >> (8 * ks));
+          } else {
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
-        }
-        float sum = 0.f;
+            for (int ks = 0; ks < 2; ++ks) {
+              const E8 pb = acc_to<EL>(sc, ks);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sc[e] = fast_exp2(fmaf(sc[e], c, -base));
-          sum += sc[e];
-        }
-        l_run += sum;
-        // rows that are not written (p = -1) need no care
-        const bool edge = __ballot(p >= 0 && seen != 0xffffu) != 0;
-        if (edge && !paged_tile_finite<EL, D, 2>(rd, vt)) {
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks)
-            paged_pv_guarded<EL, D>(oacc, rd, vt, ks, acc_to<EL>(sc, ks), seen >> (8 * ks));
-        } else {
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            const E8 pb = acc_to<EL>(sc, ks);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) oacc[dt] = mfma32(op[DT * ks + dt], pb, oacc[dt]);
+              for (int dt = 0; dt < DT; ++dt) oacc[dt] = mfma32(op[DT * ks + dt], pb, oacc[dt]);
+            }
           }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_sched_barrier(0);
+          issue(SLOTS & 1 ? dk : dv, ring + at * TILE, t + (SLOTS + 1) / 2, !(SLOTS & 1));
+          at = at + 1 == SLOTS ? 0 : at + 1;
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        issue(SLOTS & 1 ? dk : dv, ring + at * TILE, t + (SLOTS + 1) / 2, !(SLOTS & 1));
-        at = at + 1 == SLOTS ? 0 : at + 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (guard || !paged_any_nan<DT>(oacc, valid)) break;
+        guard = true;
       }
       // join the waves
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       const float l_tot = valid ? pair_sum(l_run) : 0.f;
       if (!valid) m_run = -INFINITY;
       __syncthreads();  // every wave is done with its slots

@@ -197,7 +197,7 @@ void paged_tile_kernel(const PagedArgs a) {
 
   // zero rows: tokens that are not selected and those of no sequence, a slice of them a
   // workgroup, D / 8 lanes a row
-  if (a.sel != nullptr || a.zero_rest) {
+  if (a.sel != nullptr || (a.zero_rest && (a.c.cu[0] > 0 || a.c.cu[a.c.nseq] < a.n))) {
     constexpr int CH = D / 8;
     const int slices = (int)(gridDim.x / a.c.heads), per = (int)((a.n + slices - 1) / slices);
     const int64_t n0 = (int64_t)rank * per, first = a.c.cu[0], end = a.c.cu[a.c.nseq];
@@ -214,11 +214,14 @@ void paged_tile_kernel(const PagedArgs a) {
   const PagedSeq s(a, w.b);
   const int r0 = w.tile * ROWS, pos0 = s.len - s.nq;
   // token in the sequence of row r
-  auto token = [&](int r) { return a.sel ? a.idx[s.lo + r / a.g] : r / a.g; };
+  auto token = [&](int r) {
+    const int t = a.g == 1 ? r : (int)((uint32_t)r / (uint32_t)a.g);
+    return a.sel ? a.idx[s.lo + t] : t;
+  };
   const int rl = min(r0 + ROWS, w.rows) - 1;  // last row
   const int wr = r0 + 32 * wave, r = min(wr + i, rl);
   const bool valid = wr + i <= rl, active = wr <= rl;
-  const int tok = token(r), hrow = r % a.g;   // and its query head in the group
+  const int tok = token(r), hrow = a.g == 1 ? 0 : r % a.g;   // and its query head in the group
   const int p = valid ? pos0 + tok : -1;
   // held as lane values: with scalar branches around the pipelined bodies the register
   // allocator spills hundreds of values between them
@@ -241,16 +244,11 @@ void paged_tile_kernel(const PagedArgs a) {
     const bf16* const qrow = a.q + (s.lo + tok) * a.q_token + (h * a.g + hrow) * a.q_head + 8 * g;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) qreg[ds] = valid ? *reinterpret_cast<const E8*>(qrow + 16 * ds) : E8{};
-    // they have arrived here: waited for inside the loop, they would drain its copies each time
-#pragma unroll
-    for (int ds = 0; ds < DS; ++ds) pin(qreg[ds]);
   }
   f32x16 oacc[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
   f32x16 sbuf[2][2];  // [t & 1][32-key half]: scores of this tile and the next
   E8 pb[4];           // P(t) as the PV MFMAs' operand
-  float m_run = -INFINITY, l_run = 0.f, base = 0.f;
+  float m_run, l_run, base;
   const float c = a.scale_log2;
 
   TileReader<D, kSwz> rd;  // K read along rows, V transposed
@@ -269,6 +267,7 @@ void paged_tile_kernel(const PagedArgs a) {
   int page_v = -1;              // page of the wave's rows of tile t + 1
   uint32_t bad1 = 0, bad2 = 0;  // groups without a page of tiles t + 1 and t + 2
   bool edge = false;            // tile t crosses the edge of some row's keys
+  bool guard = false;           // a second run, for values that are not finite behind an edge
 
   auto step = [&](auto par_tag, int t) {
     constexpr int PAR = decltype(par_tag)::value;  // t & 1
@@ -379,8 +378,8 @@ void paged_tile_kernel(const PagedArgs a) {
     using F_ = std::false_type;
     const bool doS = t + 1 >= tw_lo && t + 1 < tw_hi;
     bool doPV = t >= tw_lo && t < tw_hi;
-    if (doPV && edge && !paged_tile_finite<EL, D, 4>(rd, vb)) {
-      // values that are not finite under a mask: this tile by itself
+    if (guard && doPV && edge) {
+      // this tile by itself
       const int hi = p - (j0n - 64) - 4 * g;
       uint32_t bad0;
       pages.get(t, bad0);
@@ -413,16 +412,33 @@ void paged_tile_kernel(const PagedArgs a) {
     __syncthreads();
   };
 
-  if (nt > 0) {
-    page_v = pages.get(0, bad2);
-    load(dk, tileK(0), 0, page_v);
-    wait_vmem();
-    __syncthreads();
-    // step -1 copies V(0) and K(1)
-    for (int t = -1; t < nt; t += 2) {
-      step(std::integral_constant<int, 1>{}, t);
-      if (t + 1 < nt) step(std::integral_constant<int, 0>{}, t + 1);
+  __shared__ int redo;
+#pragma unroll 1
+  for (;;) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
+    m_run = -INFINITY, l_run = base = 0.f;
+    if (nt > 0) {
+      page_v = pages.get(0, bad2);
+      load(dk, tileK(0), 0, page_v);
+      if (tid == 0) redo = 0;
+      // q has arrived here too: waited for inside the loop, it would drain its copies each time
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) pin(qreg[ds]);
+      wait_vmem();
+      __syncthreads();
+      // step -1 copies V(0) and K(1)
+      for (int t = -1; t < nt; t += 2) {
+        step(std::integral_constant<int, 1>{}, t);
+        if (t + 1 < nt) step(std::integral_constant<int, 0>{}, t + 1);
+      }
     }
+    if (guard || nt == 0) break;
+    if (paged_any_nan<DT>(oacc, valid) && l == 0) redo = 1;
+    __syncthreads();
+    if (redo == 0) break;
+    guard = true;
+    __syncthreads();
   }
   const float l_tot = pair_sum(l_run);
   if (w.npiece > 1) {
