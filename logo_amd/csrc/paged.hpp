@@ -38,7 +38,7 @@ struct PagedArgs {
   const uint8_t* sel;    // [n] or null: every token
   int32_t* idx;          // [n] with sel (many rows): the selected tokens of each sequence, from its first token's place on
   int32_t* count;        // [nseq] with sel (many rows): how many
-  float* part;           // partial results, D + 2 floats a row (O unnormalised, its reference maximum, its sum)
+  float* part;           // partial results, paged_part_row(D) floats a row
   int64_t n;
   int hq, g, shift, window;
   float scale_log2;
@@ -48,6 +48,9 @@ struct PagedArgs {
   int cap;               // many rows: pieces per kv head that part holds
   int part_rows;         // rows of a piece in part
 };
+
+// A row's partial result: O unnormalised, its reference maximum, its sum (16-byte aligned).
+__host__ __device__ constexpr int paged_part_row(int d) { return d + 4; }
 
 constexpr int kPagedPad = 4;  // floats between the rows of an LDS block of partial outputs
 

@@ -48,6 +48,9 @@ namespace logo {
 constexpr int kFewWaves = 2;
 constexpr int kFewUnit = 64;      // keys
 constexpr int kFewMinShare = 4;   // units: the shortest stretch, unless a sequence ends
+// Keys up to which no sequence is cut.  One workgroup takes 8.1 us for 64 keys, 11.8 for
+// 256, 27.5 for 1024; cut in four, 1024 take 12.9 us and the launch that joins them 4.1.
+constexpr int kFewWhole = 512;
 
 template <int D>
 constexpr int few_slots() { return D == 128 ? 5 : 10; }
@@ -139,12 +142,25 @@ void paged_few_kernel(const PagedArgs a) {
 
   FewCut cut;
   int pos = 0, end = 0, rest = -1, h = 0, n = 0;
+  const bool direct = !a.split && a.c.heads * (int64_t)a.c.nseq <= gridDim.x;
 #pragma unroll 1
   for (;; pos += n, rest += n) {
     if (pos >= end && rest >= 0) return;
-    if (rest >= 0 && rest == cut.total) ++h, rest = 0;
-    cut.pass(a, rest);
-    if (rest < 0) {  // the first pass: the stretch
+    if (direct) {  // a sequence and kv head each, nothing to look for
+      if (w >= a.c.heads * a.c.nseq) return;
+      h = (uint32_t)w / (uint32_t)a.c.nseq;
+      cut.b = w - h * a.c.nseq;
+      cut.units = 1;
+      cut.start = rest = pos = 0;
+      end = 1;
+      const PagedSeq s(a, cut.b);
+      if (s.nq == 0) return;
+      cut.lo = a.window >= 0 ? max(0, s.len - s.nq - a.window) & ~(kFewUnit - 1) : 0;
+    } else if (rest >= 0) {
+      if (rest == cut.total) ++h, rest = 0;
+      cut.pass(a, rest);
+    } else {  // the first pass: the stretch
+      cut.pass(a, -1);
       const int all = cut.total * a.c.heads;
       // the last one may end before it starts
       if ((int64_t)w * cut.share >= all) return;
@@ -349,9 +365,9 @@ void paged_few_kernel(const PagedArgs a) {
           *reinterpret_cast<E8*>(a.out + ((s.lo + tk) * a.hq + h * a.g + (r0 + rr - tk * a.g)) * D + 8 * ch) = v;
         } else {
           // a stretch has one sequence that started before it and one that goes on behind it at most
-          float* const pp = a.part + ((int64_t)(2 * w + (f == 0 ? 1 : 0)) * a.part_rows + rr) * (D + 2);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) pp[8 * ch + k] = o[k];
+          float* const pp = a.part + ((int64_t)(2 * w + (f == 0 ? 1 : 0)) * a.part_rows + rr) * paged_part_row(D);
+          *reinterpret_cast<f32x4*>(pp + 8 * ch) = f32x4{o[0], o[1], o[2], o[3]};
+          *reinterpret_cast<f32x4*>(pp + 8 * ch + 4) = f32x4{o[4], o[5], o[6], o[7]};
           if (ch == 0) pp[D] = m, pp[D + 1] = lsum;
         }
       }
@@ -392,7 +408,7 @@ __global__ __launch_bounds__(256) void paged_few_join_kernel(const PagedArgs a, 
   const int np = 1 + (cut.units - f + cut.share - 1) / cut.share;
   constexpr int CL = D / 4, GR = 256 / CL;
   const int ch = tid % CL, gr = tid / CL;
-  auto part = [&](int k) { return a.part + ((int64_t)(2 * (w - 1 + k) + (k == 0 ? 1 : 0)) * a.part_rows + row) * (D + 2); };
+  auto part = [&](int k) { return a.part + ((int64_t)(2 * (w - 1 + k) + (k == 0 ? 1 : 0)) * a.part_rows + row) * paged_part_row(D); };
   __shared__ float red[4];
   __shared__ float so[GR][D + 4];
   float m = -INFINITY;
@@ -410,8 +426,9 @@ __global__ __launch_bounds__(256) void paged_few_join_kernel(const PagedArgs a, 
     const float* const q = part(k);
     const float x = fast_exp2(q[D] - base);
     ls = fmaf(x, q[D + 1], ls);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(q + 4 * ch);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(x, q[4 * ch + e], o[e]);
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(x, y[e], o[e]);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) so[gr][4 * ch + e] = o[e];
@@ -442,7 +459,7 @@ static PagedPlan paged_plan(int nseq, int h, int hq, int64_t n, int d, int max_q
   const int64_t span = window >= 0 ? std::min<int64_t>(max_len, (int64_t)window + max_q) : max_len;
   int64_t parts;
   if (p.few) {
-    p.split = span > kFewUnit * kFewMinShare;
+    p.split = span > kFewWhole;
     p.target = cus * (int)(160 * 1024 / (d == 128 ? few_smem<128>() : few_smem<64>()));
     p.part_rows = std::max(1, max_q * g);
     parts = 2 * p.target;
@@ -451,7 +468,7 @@ static PagedPlan paged_plan(int nseq, int h, int hq, int64_t n, int d, int max_q
     p.part_rows = 32 * p.nw;
     parts = (int64_t)p.cap * h;
   }
-  if (p.split) p.part_bytes = ((size_t)parts * p.part_rows * (d + 2) * sizeof(float) + 255) & ~(size_t)255;
+  if (p.split) p.part_bytes = ((size_t)parts * p.part_rows * paged_part_row(d) * sizeof(float) + 255) & ~(size_t)255;
   p.bytes = p.part_bytes + (sel && !p.few ? ((size_t)n + nseq) * sizeof(int32_t) : 0);
   return p;
 }

@@ -51,56 +51,86 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedAr
   if (tid == 0) a.count[b] = done;
 }
 
-// The cut of a launch's rows and keys.  Where the row tiles of all kv heads fill less
-// than three quarters of the workgroups that the device holds (a.target), each tile's
-// keys are cut into pieces, up to two rounds of workgroups in all, of equal size for all
-// sequences (the longest one's keys over their number).  Every workgroup works out the
-// same from cu, lens and the selected tokens' counts.
+// The cut of a launch's rows and keys.  Where the row tiles leave the device idle, each
+// tile's keys are cut into pieces of equal size for all sequences.  How many: a launch
+// lasts about as many rounds of workgroups as its pieces fill, each as long as a full
+// piece with what a workgroup costs beside (kPieceCost, in keys: its start, its partial
+// results); the number with the shortest sum is taken.  Every workgroup works out the
+// same from cu, lens and the selected tokens' counts.  Against pieces for two rounds
+// wherever the tiles fill less than three quarters of one: 512 tokens behind 7680 (16
+// heads over 4, D = 128) 79 -> 59 us, four of them 164 -> 155, a quarter of 8192 tokens
+// behind 24576 (16 heads) 640 -> 560; twelve single tokens beside four such chunks the same.
 constexpr int kMaxPieces = 16;
 constexpr int kTileMinChunk = 512;  // keys
+constexpr float kPieceCost = 400.f;
 
 struct TileWork {
   int b, tile, rows;   // sequence, row tile, the sequence's rows
   int npiece, chunk;   // pieces a row tile, keys a piece
   int piece;
-  __device__ __forceinline__ static int rows_of(const PagedArgs& a, int b, int& len) {
-    len = 0;
+  __device__ __forceinline__ static int rows_of(const PagedArgs& a, int b, int& len, int& nq) {
+    len = nq = 0;
     if (b >= a.c.nseq) return 0;
     const PagedSeq s(a, b);
     len = s.len;
+    nq = s.nq;
     return max(0, a.sel ? min(a.count[b], s.nq) : s.nq) * a.g;
   }
   // The rank-th (row tile, piece) of a kv head, the latest rows of a sequence first (they see the most keys); with
   // pieces = false the rank-th row tile.  By a whole wave; false: none.
   __device__ __forceinline__ bool find(const PagedArgs& a, int rank, int tile_rows, bool pieces) {
     const int lane = threadIdx.x & 63;
-    int len, r = rows_of(a, lane, len), nt = (r + tile_rows - 1) / tile_rows;
+    int len, nq, r = rows_of(a, lane, len, nq), nt = (r + tile_rows - 1) / tile_rows;
     npiece = 1;
     chunk = 0x7fffffff;
     if (a.split) {
       int total = nt, longest = nt > 0 ? len : 0;
+      float keys = nt * (len - 0.5f * nq);  // of all tiles, about
       for (int c = 64; c < a.c.nseq; c += 64) {
-        int x;
-        const int k = (rows_of(a, c + lane, x) + tile_rows - 1) / tile_rows;
+        int x, y;
+        const int k = (rows_of(a, c + lane, x, y) + tile_rows - 1) / tile_rows;
         total += k;
         if (k > 0) longest = max(longest, x);
+        keys += k * (x - 0.5f * y);
       }
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) {
         total += __shfl_xor(total, off);
         longest = max(longest, __shfl_xor(longest, off));
+        keys += __shfl_xor(keys, off);
       }
-      total = uniform(total);
-      longest = uniform(longest);
-      const int wgs = max(1, total * a.c.heads);
-      if (4 * wgs < 3 * a.target && a.window < 0) {
-        npiece = max(1, min(min(2 * a.target / wgs, kMaxPieces), longest / kTileMinChunk));
-        if (npiece > 1) chunk = ((longest + npiece - 1) / npiece + 127) & ~127;
+      const float wgs = (float)total * a.c.heads;
+      // a lane a number of pieces; the partial results have room for 2 a.target
+      const int n = lane % kMaxPieces + 1, size = ((longest + n - 1) / n + 127) & ~127;
+      const bool fits = n == 1 || (size >= kTileMinChunk && n * wgs <= 2.f * a.target);
+      const float per_key = __builtin_amdgcn_rcpf((float)size);
+      float count = keys * per_key + 0.5f * total;
+      if (a.c.nseq <= 16) {  // few sequences: counted, by the pieces of a middle row
+        const float middle = len - 0.5f * nq;
+        count = 0.f;
+        for (int k = 0; k < a.c.nseq; ++k) {
+          const int x = __builtin_amdgcn_readlane(__float_as_int(middle), k);
+          count = fmaf((float)__builtin_amdgcn_readlane(nt, k), ceilf(__int_as_float(x) * per_key), count);
+        }
       }
+      count = n == 1 ? wgs : count * a.c.heads;
+      // whole rounds where the tiles are about as long as the longest; others end one by one
+      const float rounds = count * __builtin_amdgcn_rcpf((float)a.target);
+      const float lasts = keys > 0.8f * total * longest ? ceilf(rounds) : fmaxf(1.f, rounds + 0.5f);
+      float cost = fits ? lasts * (size + kPieceCost) : INFINITY;
+      int best = n;
+#pragma unroll
+      for (int off = kMaxPieces / 2; off > 0; off >>= 1) {
+        const float o = __shfl_xor(cost, off);
+        const int ob = __shfl_xor(best, off);
+        if (o < cost || (o == cost && ob < best)) cost = o, best = ob;
+      }
+      npiece = a.window < 0 ? uniform(best) : 1;
+      if (npiece > 1) chunk = ((uniform(longest) + npiece - 1) / npiece + 127) & ~127;
     }
     const int per = pieces ? npiece : 1;
     for (int c = 0; c < a.c.nseq; c += 64) {
-      if (c > 0) r = rows_of(a, c + lane, len), nt = (r + tile_rows - 1) / tile_rows;
+      if (c > 0) r = rows_of(a, c + lane, len, nq), nt = (r + tile_rows - 1) / tile_rows;
       int pre = nt * per;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
@@ -443,11 +473,16 @@ void paged_tile_kernel(const PagedArgs a) {
   const float l_tot = pair_sum(l_run);
   if (w.npiece > 1) {
     if (valid) {
-      float* const pp = a.part + (((int64_t)h * a.cap + rank) * ROWS + 32 * wave + i) * (D + 2);
+      float* const pp = a.part + (((int64_t)h * a.cap + rank) * ROWS + 32 * wave + i) * paged_part_row(D);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pp[32 * dt + rowmap(g, e)] = oacc[dt][e];
+        for (int q4 = 0; q4 < 4; ++q4) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = oacc[dt][4 * q4 + e];
+          *reinterpret_cast<f32x4*>(pp + 32 * dt + 8 * q4 + 4 * g) = v;
+        }
       if (g == 0) pp[D] = m_run, pp[D + 1] = l_tot;
     }
     return;
@@ -492,9 +527,9 @@ __global__ __launch_bounds__(256) void paged_tile_join_kernel(const PagedArgs a)
   const int tok = a.sel ? a.idx[s.lo + r / a.g] : r / a.g, p = s.len - s.nq + tok;
   // pieces that hold keys which the row sees
   const int np = p < 0 ? 0 : min(p / w.chunk, w.npiece - 1) + 1;
-  const int64_t step = (int64_t)ROWS * (D + 2);
+  const int64_t step = (int64_t)ROWS * paged_part_row(D);
   const float* const pp = a.part + ((int64_t)h * a.cap + (blockIdx.x / (ROWS / kJoinRows)) * w.npiece) * step +
-                          (r - w.tile * ROWS) * (D + 2);
+                          (r - w.tile * ROWS) * paged_part_row(D);
   float m = -INFINITY;
   for (int k = 0; k < np; ++k) m = fmaxf(m, pp[k * step + D]);
   const float base = m == -INFINITY ? 0.f : m;
@@ -503,8 +538,9 @@ __global__ __launch_bounds__(256) void paged_tile_join_kernel(const PagedArgs a)
   for (int k = 0; k < np; ++k) {
     const float f = fast_exp2(pp[k * step + D] - base);
     sum = fmaf(f, pp[k * step + D + 1], sum);
+    const fv x = *reinterpret_cast<const fv*>(pp + k * step + col);
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = fmaf(f, pp[k * step + col + e], o[e]);
+    for (int e = 0; e < V; ++e) o[e] = fmaf(f, x[e], o[e]);
   }
   ev v;
 #pragma unroll
@@ -549,7 +585,7 @@ void tile_plan(int nseq, int h, int g, int64_t n, int64_t span, int cus, bool se
   nw = !sel && rows / 256 * h >= 2 * cus ? 8 : 4;
   target = cus * 8 / nw;
   // the selected rows may be few of all, else the row tiles are known but for the sequences' ends
-  split = span >= 2 * kTileMinChunk && (sel || 4 * (rows / (32 * nw)) * h < 3 * (int64_t)target);
+  split = span >= 2 * kTileMinChunk && (sel || rows / (32 * nw) * h < (int64_t)target);
   const int64_t tiles = rows / (32 * nw) + nseq;
   cap = split ? (int)std::max<int64_t>(1, std::min<int64_t>(2 * target / h, tiles * kMaxPieces)) : 0;
 }
