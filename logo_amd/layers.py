@@ -31,6 +31,7 @@ from .ops.decode import LogoKVCache, decode_attn, decode_attn_fused, decode_qkv
 from .ops.epilogue import logo_epilogue
 from .ops.glue import (attn_inputs, dec_linear, dec_linear_faster, dec_linear_ok, global_maps_, global_maps_ok,
                        head_linear, head_proj, rms_norm, rope, rope_apply_, silu_mul)
+from .ops.paged import PagedLogoCache, PagedStep, paged_append, paged_attn
 from .ops.sq_attn import dense_causal_attn, sq_full_attn, swa_attn
 
 __all__ = ["LoGoConfig", "LoGoAttention", "Attention", "RMSNorm", "rope_cos_sin", "apply_rope", "position_ids_for"]
@@ -544,6 +545,25 @@ class LoGoAttention(nn.Module):
         return self._fuse(local.view(B, 1, H, D), glob.view(B, 1, H, D), gate.view(B, 1))
 
 
+    def paged(self, h, cache: PagedLogoCache, step: PagedStep):
+        """The layer on a step's packed tokens ``h [N, C]`` (no gradients): keys and
+        values of both branches go to the cache's pages, rotated by their positions,
+        and each token attends its own sequence's (logo/layers/logo.py:112-258), the
+        global branch for the tokens that the gate selects."""
+        N, H, HK, D, li = h.shape[0], self.num_heads, self.num_key_value_heads, self.head_dim, self.layer_idx
+        q, k, v = self.q_proj(h).view(N, H, D), self.k_proj(h).view(N, HK, D), self.v_proj(h).view(N, HK, D)
+        gq, gk, gv = (x[0] for x in self._global_qkv(q[None], k[None], v[None]))
+        gate = torch.sigmoid(self.gate_proj(h))  # [N, 1]
+        local = (cache.local_k[li], cache.local_v[li], step.local_table, step.cu, step.lens)
+        pages = (cache.global_k[li], cache.global_v[li], step.table, step.cu, step.lens)
+        q = paged_append(k, v, *local, q=q, plan=cache.rotary)
+        gq = paged_append(gk, gv, *pages, q=gq, plan=cache.rotary)
+        bounds = dict(max_q=step.max_q, max_len=step.max_len)
+        loc = paged_attn(q, *local, window=self.local_window_size, **bounds)
+        glob = paged_attn(gq, *pages, selection=(gate >= self.gate_thres).view(N), **bounds)
+        return self.o_proj(self._fuse(loc[None], glob[None], gate[None])[0])
+
+
 class Attention(nn.Module):
     """Plain causal attention layer, used where ``attn_type_list[i] != 0``
     (logo/layers/attn.py:22-127, selected at logo/modeling_logo.py:47-51):
@@ -603,3 +623,12 @@ class Attention(nn.Module):
             out = plan.unpack(dense_causal_attn(plan.pack(q), plan.pack(k), plan.pack(v), plan.cu), B, T)
             out = out.reshape(B, T, H * D)
         return self.o_proj(out), None, past_key_value
+
+    def paged(self, h, cache: PagedLogoCache, step: PagedStep):
+        """The layer on a step's packed tokens ``h [N, C]`` (no gradients), its keys
+        and values in the cache's global pages."""
+        N, H, HK, D, li = h.shape[0], self.num_heads, self.num_key_value_heads, self.head_dim, self.layer_idx
+        pages = (cache.global_k[li], cache.global_v[li], step.table, step.cu, step.lens)
+        q = paged_append(self.k_proj(h).view(N, HK, D), self.v_proj(h).view(N, HK, D), *pages,
+                         q=self.q_proj(h).view(N, H, D), plan=cache.rotary)
+        return self.o_proj(paged_attn(q, *pages, max_q=step.max_q, max_len=step.max_len).view(N, H * D))

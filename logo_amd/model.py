@@ -25,6 +25,7 @@ from .layers import (Attention, LoGoAttention, LoGoConfig, RMSNorm, _fused_ok, _
                      padding_mask, position_ids_for, rope_cos_sin, rows_product)
 from .ops.decode import LogoKVCache
 from .ops.glue import DEC_LINEAR_MAX_ROWS, add_rms_norm, silu_mul
+from .ops.paged import PagedLogoCache, PagedStep
 
 __all__ = ["LoGoMLP", "LoGoDecoderLayer", "LoGoModel", "LoGoForCausalLM"]
 
@@ -165,6 +166,26 @@ class LoGoModel(nn.Module):
         return self.norm(h)
 
 
+    def paged(self, input_ids, cache: PagedLogoCache, step: PagedStep):
+        """Hidden states ``[N, C]`` of a step's packed tokens ``[N]``, over the cache
+        (no gradients)."""
+        h = self.embed_tokens(input_ids)
+        fused = _fused_ok(h) and h.shape[-1] <= 4096
+        normed = self.layers[0].input_layernorm(h) if len(self.layers) else self.norm(h)
+        for i, layer in enumerate(self.layers):
+            pn = layer.post_attention_layernorm
+            nn_ = self.layers[i + 1].input_layernorm if i + 1 < len(self.layers) else self.norm
+            # each residual add with the norm that follows it
+            for part, norm in ((lambda x: layer.self_attn.paged(x, cache, step), pn), (layer.mlp, nn_)):
+                x = part(normed)
+                if fused:
+                    h, normed = add_rms_norm(h, x, norm.weight, norm.variance_epsilon)
+                else:
+                    h = h + x
+                    normed = norm(h)
+        return normed
+
+
 class LoGoForCausalLM(nn.Module):
     """Causal LM head over ``LoGoModel`` (logo/modeling_logo.py:308-380)."""
 
@@ -238,6 +259,24 @@ class LoGoForCausalLM(nn.Module):
         logits = self.forward(tokens[:, None], past_key_value=cache, last_only=True)
         cache.advance()
         return logits
+
+    def new_paged_cache(self, pages: int, local_pages: Optional[int] = None, page_size: int = 64,
+                        device=None) -> PagedLogoCache:
+        """A paged cache for ``paged_step``, its pages of the model's type."""
+        c = self.config
+        return PagedLogoCache(c.num_hidden_layers, c.num_key_value_heads, c.head_dim, pages, local_pages, page_size,
+                              window=c.window_size, rope_theta=c.rope_theta, dtype=self.lm_head.weight.dtype,
+                              device=device)
+
+    @torch.no_grad()
+    def paged_step(self, input_ids, cache: PagedLogoCache, step: PagedStep):
+        """One step of a server over ``step.seqs``: their new tokens ``input_ids
+        [N]``, packed, prompts in pieces of any size beside single tokens.  Returns
+        the logits ``[S, V]`` of each sequence's last token."""
+        if input_ids.dim() != 1 or input_ids.shape[0] != sum(step.new):
+            raise ValueError(f"paged_step: input_ids must be [{sum(step.new)}], got {tuple(input_ids.shape)}")
+        h = self.model.paged(input_ids, cache, step)
+        return linear_rows(self.lm_head, h.index_select(0, step.last))
 
     @torch.no_grad()
     def capture_greedy_decode(self, tokens, cache: LogoKVCache):
