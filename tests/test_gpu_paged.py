@@ -303,3 +303,135 @@ def test_append_then_attend(gpu):
         # a rotated value that fp32 puts on the other side of a rounding border is off by a whole step: at most a few,
         # each moving a score by 2^-7 of one of 64 products
         ref.check("o", torch.cat(outs[s]), r, ref.attn_bound(r, mag, BF16) + 2.0 ** -8 * mag)
+
+
+@pytest.mark.parametrize("big", [False, True])
+def test_many_sequences(gpu, big):
+    """More sequences than a wave has lanes (and than the pieces are counted for), many of them empty."""
+    g = gen(19)
+    S = 150
+    new = [0 if s % 4 == 3 else 1 + (s * 7) % (40 if big else 5) for s in range(S)]
+    lens = [n + (s * 37) % 300 if s % 11 else n for s, n in enumerate(new)]
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 1, 64, 16, BF16, g)
+    N = sum(new)
+    q = torch.randn(N, 4, 64, generator=g).bfloat16()
+    sel = torch.rand(N, generator=g) < 0.5
+    args = [t.to(gpu) for t in (kp, vp, table, cu, ln)]
+    for kw in (dict(), dict(window=30), dict(selection=sel)):
+        r, mag = ref.paged_attn(q, kp, vp, table, cu, ln, **kw)
+        kw = {k: v.to(gpu) if torch.is_tensor(v) else v for k, v in kw.items()}
+        for bounds in (dict(max_q=max(new), max_len=max(lens)), dict(max_q=5, max_len=5000), dict()):
+            o = paged_attn(q.to(gpu), *args, **kw, **bounds)
+            ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
+
+
+@pytest.mark.parametrize("bounds", [dict(max_q=1, max_len=3000), dict(max_q=8, max_len=16), dict(max_q=100, max_len=1),
+                                    dict(max_q=0, max_len=0), dict(max_q=100000, max_len=1 << 40)])
+def test_wrong_bounds_cost_time_only(gpu, bounds):
+    g = gen(20)
+    new, lens = [40, 1, 9], [1500, 2999, 700]
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 2, 64, 32, F16, g)
+    q = torch.randn(sum(new), 8, 64, generator=g).half()
+    sel = torch.rand(sum(new), generator=g) < 0.6
+    r, mag = ref.paged_attn(q, kp, vp, table, cu, ln, selection=sel)
+    o = paged_attn(q.to(gpu), *[t.to(gpu) for t in (kp, vp, table, cu, ln)], selection=sel.to(gpu), **bounds)
+    ref.check("o", o, r, ref.attn_bound(r, mag, F16))
+
+
+def test_pages_beyond_32_bits(gpu):
+    """Pages 3 GB apart: element and byte offsets past 2^32."""
+    D, H, page, stride = 64, 2, 16, 3 << 29
+    pools = [torch.empty(2 * stride + H * page * D, dtype=BF16, device=gpu).as_strided(
+        (3, H, page, D), (stride, page * D, D, 1)) for _ in range(2)]
+    g = gen(21)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32)
+    cu, ln = torch.tensor([0, 40], dtype=torch.int32), torch.tensor([40], dtype=torch.int32)
+    q, k, v = (torch.randn(40, h, D, generator=g).bfloat16() for h in (4, H, H))
+    args = [*pools, table.to(gpu), cu.to(gpu), ln.to(gpu)]
+    assert paged_append(k.to(gpu), v.to(gpu), *args) is None
+    small = [torch.zeros(3, H, page, D, dtype=BF16) for _ in range(2)]
+    for j in range(40):
+        p = int(table[0, j // page])
+        small[0][p, :, j % page], small[1][p, :, j % page] = k[j], v[j]
+        assert torch.equal(pools[0][p, :, j % page].cpu(), k[j])
+    r, mag = ref.paged_attn(q, *small, table, cu, ln)
+    ref.check("chunk", paged_attn(q.to(gpu), *args, max_q=40, max_len=40), r, ref.attn_bound(r, mag, BF16))
+    r, mag = r[39:], mag[39:]
+    one = torch.tensor([0, 1], dtype=torch.int32, device=gpu)
+    o = paged_attn(q[39:].to(gpu), *args[:3], one, args[4], max_q=1, max_len=40)
+    ref.check("token", o, r, ref.attn_bound(r, mag, BF16))
+
+
+def test_shared_pages_and_repeated_runs(gpu):
+    """Two sequences with a common prefix in the same pages; the same call gives the same bits."""
+    g = gen(22)
+    kp, vp, table, cu, ln = ref.paged_inputs([3, 5], [800, 700], 2, 128, 64, BF16, g)
+    table[1, :9] = table[0, :9]
+    q = torch.randn(8, 6, 128, generator=g).bfloat16()
+    r, mag = ref.paged_attn(q, kp, vp, table, cu, ln)
+    args = [t.to(gpu) for t in (kp, vp, table, cu, ln)]
+    for bounds in (dict(max_q=5, max_len=800), dict(max_q=50, max_len=800)):
+        o = paged_attn(q.to(gpu), *args, **bounds)
+        ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
+        for _ in range(5):
+            assert torch.equal(o, paged_attn(q.to(gpu), *args, **bounds))
+
+
+def test_append_captured_with_attention(gpu):
+    """A decode step's append and attention in one graph, replayed as the lengths grow on the device."""
+    D, H, HQ, page = 128, 2, 4, 16
+    g = gen(23)
+    plan = rotary_plan(D, rot_dim=64, interleaved=True, device=gpu)
+    lens0 = [200, 5]
+    kp, vp, table, _, ln = ref.paged_inputs([0, 0], lens0, H, D, page, BF16, g, spare=8)
+    free = sorted(set(range(kp.shape[0])) - set(table.flatten().tolist()))
+    table = torch.cat([table[:, :13], torch.full((2, 1), -1, dtype=torch.int32)], dim=1)
+    table[0, 13], table[1, 1] = free[0], free[1]
+    rows = torch.randn(2, (HQ + 2 * H) * D, generator=g).bfloat16().to(gpu)
+    q, k, v = (t.unflatten(1, (-1, D)) for t in rows.split((HQ * D, H * D, H * D), dim=1))
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=gpu)
+    twins = [[t.to(gpu) for t in (kp, vp, table, ln)] for _ in range(2)]
+
+    def step(t):
+        t[3].add_(1)
+        qr = paged_append(k, v, t[0], t[1], t[2], cu, t[3], q=q, plan=plan)
+        return paged_attn(qr, t[0], t[1], t[2], cu, t[3], max_q=1, max_len=220)
+
+    side = torch.cuda.Stream(device=gpu)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = [t.clone() for t in twins[0]]
+        step(warm)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step(twins[0])
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(12):
+        graph.replay()
+        eager = step(twins[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and bool(out.isfinite().all())
+        rows.mul_(0.9)
+    for a, b in zip(*twins):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+def test_operator_registrations(gpu):
+    """torch.library's checks of the operators: schemas, fakes, autograd registration."""
+    from logo_amd import _torch_ops
+
+    ops = _torch_ops.ops()
+    g = gen(24)
+    kp, vp, table, cu, ln = (t.to(gpu) for t in ref.paged_inputs([3, 40], [30, 90], 1, 64, 16, BF16, g))
+    kp, vp = kp.nan_to_num(), vp.nan_to_num()
+    q = torch.randn(43, 2, 64, generator=g).bfloat16().to(gpu)
+    k = torch.randn(43, 1, 64, generator=g).bfloat16().to(gpu)
+    plan = rotary_plan(64, device=gpu)
+    rot = (plan.turns, 64, 64, False, 1.0)
+    check = torch.library.opcheck
+    check(ops.paged_attn, (q, kp, vp, table, cu, ln, None, 40, 90, 0.125, -1))
+    check(ops.paged_attn_out, (q, kp, vp, table, cu, ln, None, 40, 90, 0.125, -1, torch.empty_like(q)))
+    check(ops.paged_append, (k, k.clone(), kp, vp, table, cu, ln, q, *rot))
+    check(ops.paged_append, (k, k.clone(), kp, vp, table, cu, ln, None, None, 0, 0, False, 1.0))
+    check(ops.rotary, ([q.float().requires_grad_()], torch.arange(43, device=gpu), *rot, False))
+    check(ops.rotary_, ([q.clone()], torch.arange(43, device=gpu), *rot))
