@@ -63,11 +63,12 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedAr
 constexpr int kMaxPieces = 16;
 constexpr int kTileMinChunk = 512;  // keys
 constexpr float kPieceCost = 400.f;
+constexpr int kPieceRounds = 2;  // pieces that the partial results have room for, in rounds of workgroups
 
 struct TileWork {
   int b, tile, rows;   // sequence, row tile, the sequence's rows
   int npiece, chunk;   // pieces a row tile, keys a piece
-  int piece;
+  int piece, total;    // total (split): row tiles of a kv head
   __device__ __forceinline__ static int rows_of(const PagedArgs& a, int b, int& len, int& nq) {
     len = nq = 0;
     if (b >= a.c.nseq) return 0;
@@ -76,15 +77,23 @@ struct TileWork {
     nq = s.nq;
     return max(0, a.sel ? min(a.count[b], s.nq) : s.nq) * a.g;
   }
-  // The rank-th (row tile, piece) of a kv head, the latest rows of a sequence first (they see the most keys); with
-  // pieces = false the rank-th row tile.  By a whole wave; false: none.
+  // The rank-th (piece, row tile) of a kv head: first pieces of all tiles, then second
+  // ones, so that those that the ends of sequences shorten come last; the latest rows of
+  // a sequence first (they see the most keys).  With pieces = false the rank-th row tile.
+  // Against all pieces of a tile together: 1000 tokens each at the ends of 1000, 2000 and
+  // 3000 keys (16 heads, D = 128) 96 -> 78 us, a quarter of 8192 tokens behind 24576
+  // 650 -> 605, 300, 700 and 120 tokens at the ends of 5000, 9000 and 2000 keys (16 heads
+  // over 4) 115 -> 113.
+  // By a whole wave; false: none.
   __device__ __forceinline__ bool find(const PagedArgs& a, int rank, int tile_rows, bool pieces) {
     const int lane = threadIdx.x & 63;
     int len, nq, r = rows_of(a, lane, len, nq), nt = (r + tile_rows - 1) / tile_rows;
     npiece = 1;
+    piece = total = 0;
     chunk = 0x7fffffff;
     if (a.split) {
-      int total = nt, longest = nt > 0 ? len : 0;
+      int longest = nt > 0 ? len : 0;
+      total = nt;
       float keys = nt * (len - 0.5f * nq);  // of all tiles, about
       for (int c = 64; c < a.c.nseq; c += 64) {
         int x, y;
@@ -99,10 +108,11 @@ struct TileWork {
         longest = max(longest, __shfl_xor(longest, off));
         keys += __shfl_xor(keys, off);
       }
+      total = uniform(total);
       const float wgs = (float)total * a.c.heads;
-      // a lane a number of pieces; the partial results have room for 2 a.target
+      // a lane a number of pieces, as far as the partial results have room
       const int n = lane % kMaxPieces + 1, size = ((longest + n - 1) / n + 127) & ~127;
-      const bool fits = n == 1 || (size >= kTileMinChunk && n * wgs <= 2.f * a.target);
+      const bool fits = n == 1 || (size >= kTileMinChunk && n * wgs <= (float)kPieceRounds * a.target);
       const float per_key = __builtin_amdgcn_rcpf((float)size);
       float count = keys * per_key + 0.5f * total;
       if (a.c.nseq <= 16) {  // few sequences: counted, by the pieces of a middle row
@@ -128,10 +138,14 @@ struct TileWork {
       npiece = a.window < 0 ? uniform(best) : 1;
       if (npiece > 1) chunk = ((uniform(longest) + npiece - 1) / npiece + 127) & ~127;
     }
-    const int per = pieces ? npiece : 1;
+    if (pieces && npiece > 1) {
+      piece = rank / total;
+      if (piece >= npiece) return false;
+      rank -= piece * total;
+    }
     for (int c = 0; c < a.c.nseq; c += 64) {
       if (c > 0) r = rows_of(a, c + lane, len, nq), nt = (r + tile_rows - 1) / tile_rows;
-      int pre = nt * per;
+      int pre = nt;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
         const int o = __shfl_up(pre, off);
@@ -141,11 +155,10 @@ struct TileWork {
       if (past != 0) {
         const int j = __builtin_ctzll(past);
         const int tiles = __builtin_amdgcn_readlane(nt, j);
-        const int k = rank - (__builtin_amdgcn_readlane(pre, j) - tiles * per);
+        const int k = rank - (__builtin_amdgcn_readlane(pre, j) - tiles);
         b = c + j;
         rows = __builtin_amdgcn_readlane(r, j);
-        piece = k % per;
-        tile = tiles - 1 - k / per;
+        tile = tiles - 1 - k;  // the latest rows, with the most keys, first
         return true;
       }
       rank -= __builtin_amdgcn_readlane(pre, 63);
@@ -527,8 +540,8 @@ __global__ __launch_bounds__(256) void paged_tile_join_kernel(const PagedArgs a)
   const int tok = a.sel ? a.idx[s.lo + r / a.g] : r / a.g, p = s.len - s.nq + tok;
   // pieces that hold keys which the row sees
   const int np = p < 0 ? 0 : min(p / w.chunk, w.npiece - 1) + 1;
-  const int64_t step = (int64_t)ROWS * paged_part_row(D);
-  const float* const pp = a.part + ((int64_t)h * a.cap + (blockIdx.x / (ROWS / kJoinRows)) * w.npiece) * step +
+  const int64_t size = (int64_t)ROWS * paged_part_row(D), step = w.total * size;
+  const float* const pp = a.part + ((int64_t)h * a.cap + blockIdx.x / (ROWS / kJoinRows)) * size +
                           (r - w.tile * ROWS) * paged_part_row(D);
   float m = -INFINITY;
   for (int k = 0; k < np; ++k) m = fmaxf(m, pp[k * step + D]);
@@ -587,7 +600,7 @@ void tile_plan(int nseq, int h, int g, int64_t n, int64_t span, int cus, bool se
   // the selected rows may be few of all, else the row tiles are known but for the sequences' ends
   split = span >= 2 * kTileMinChunk && (sel || rows / (32 * nw) * h < (int64_t)target);
   const int64_t tiles = rows / (32 * nw) + nseq;
-  cap = split ? (int)std::max<int64_t>(1, std::min<int64_t>(2 * target / h, tiles * kMaxPieces)) : 0;
+  cap = split ? (int)std::max<int64_t>(1, std::min<int64_t>(kPieceRounds * target / h, tiles * kMaxPieces)) : 0;
 }
 
 int paged_launch_tile(const PagedArgs& a, int h, int d, bool half, int nw, hipStream_t st) {
