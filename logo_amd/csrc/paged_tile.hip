@@ -63,6 +63,7 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedAr
 constexpr int kMaxPieces = 16;
 constexpr int kTileMinChunk = 512;  // keys
 constexpr float kPieceCost = 400.f;
+constexpr int kOneByOne = 16;       // sequences up to which each is looked at for the cut and the order
 constexpr int kPieceRounds = 2;  // pieces that the partial results have room for, in rounds of workgroups
 
 struct TileWork {
@@ -115,7 +116,7 @@ struct TileWork {
       const bool fits = n == 1 || (size >= kTileMinChunk && n * wgs <= (float)kPieceRounds * a.target);
       const float per_key = __builtin_amdgcn_rcpf((float)size);
       float count = keys * per_key + 0.5f * total;
-      if (a.c.nseq <= 16) {  // few sequences: counted, by the pieces of a middle row
+      if (a.c.nseq <= kOneByOne) {  // few sequences: counted, by the pieces of a middle row
         const float middle = len - 0.5f * nq;
         count = 0.f;
         for (int k = 0; k < a.c.nseq; ++k) {
@@ -145,13 +146,26 @@ struct TileWork {
     }
     for (int c = 0; c < a.c.nseq; c += 64) {
       if (c > 0) r = rows_of(a, c + lane, len, nq), nt = (r + tile_rows - 1) / tile_rows;
-      int pre = nt;
+      // Uncut tiles of more than a round: the sequences with the longest tiles first.
+      // Against their own order: 2048 tokens each at the ends of 2048, 4096, 6144 and 8192
+      // keys (16 heads, D = 128) 312 -> 274 us (D = 64: 238 -> 198), 4096 tokens before 15
+      // single ones (16 heads over 4, 8192 keys) 334 -> 275; among 51 sequences the looking
+      // costs what it gains (349 -> 362).
+      int pre = nt;  // tiles up to the end of the lane's sequence
+      if (npiece == 1 && a.c.nseq <= kOneByOne && (!a.split || total * a.c.heads > a.target)) {
+        const int keys = 2 * len - nq;
+        for (int k = 0; k < a.c.nseq; ++k) {
+          const int x = __builtin_amdgcn_readlane(keys, k), y = __builtin_amdgcn_readlane(nt, k);
+          pre += x > keys || (x == keys && k < lane) ? y : 0;
+        }
+      } else {
 #pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int o = __shfl_up(pre, off);
-        if (lane >= off) pre += o;
+        for (int off = 1; off < 64; off <<= 1) {
+          const int o = __shfl_up(pre, off);
+          if (lane >= off) pre += o;
+        }
       }
-      const unsigned long long past = __ballot(rank < pre);
+      const unsigned long long past = __ballot(rank < pre && rank >= pre - nt);
       if (past != 0) {
         const int j = __builtin_ctzll(past);
         const int tiles = __builtin_amdgcn_readlane(nt, j);
@@ -161,7 +175,7 @@ struct TileWork {
         tile = tiles - 1 - k;  // the latest rows, with the most keys, first
         return true;
       }
-      rank -= __builtin_amdgcn_readlane(pre, 63);
+      rank -= __builtin_amdgcn_readlane(pre, 63);  // (64 sequences: past the last tile)
     }
     return false;
   }
