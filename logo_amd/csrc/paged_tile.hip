@@ -153,7 +153,7 @@ struct TileWork {
       // costs what it gains (349 -> 362).
       int pre = nt;  // tiles up to the end of the lane's sequence
       if (npiece == 1 && a.c.nseq <= kOneByOne && (!a.split || total * a.c.heads > a.target)) {
-        const int keys = 2 * len - nq;
+        const int keys = len - nq / 2;  // of a middle row
         for (int k = 0; k < a.c.nseq; ++k) {
           const int x = __builtin_amdgcn_readlane(keys, k), y = __builtin_amdgcn_readlane(nt, k);
           pre += x > keys || (x == keys && k < lane) ? y : 0;
@@ -175,7 +175,7 @@ struct TileWork {
         tile = tiles - 1 - k;  // the latest rows, with the most keys, first
         return true;
       }
-      rank -= __builtin_amdgcn_readlane(pre, 63);  // (64 sequences: past the last tile)
+      rank -= __builtin_amdgcn_readlane(pre, 63);
     }
     return false;
   }
