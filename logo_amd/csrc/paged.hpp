@@ -64,11 +64,14 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // The rows of sequence b.
 struct PagedSeq {
   int64_t lo;   // first token
-  int nq, len;  // new tokens, keys
+  int nq, len;  // new tokens, keys that the table reaches
+  int pos0;     // position of the first token
   __device__ __forceinline__ PagedSeq(const PagedArgs& a, int b) {
     lo = max(0, a.c.cu[b]);
     nq = (int)max((int64_t)0, min((int64_t)a.c.cu[b + 1], a.n) - lo);
-    len = min(max(a.c.lens[b], 0), a.c.table_width << a.shift);
+    const int all = max(a.c.lens[b], 0);
+    len = min(all, a.c.table_width << a.shift);
+    pos0 = all - nq;
   }
 };
 

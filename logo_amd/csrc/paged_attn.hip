@@ -76,7 +76,7 @@ struct FewCut {
         any = false;
         for (int t = 0; t < s.nq && !any; ++t) any = a.sel[s.lo + t] != 0;
       }
-      if (a.window >= 0) first = max(0, s.len - s.nq - a.window) & ~(kFewUnit - 1);
+      if (a.window >= 0) first = max(0, s.pos0 - a.window) & ~(kFewUnit - 1);
       n = any ? max(1, (s.len - first + kFewUnit - 1) / kFewUnit) : s.nq > 0;
     }
     pre = n;
@@ -155,7 +155,7 @@ void paged_few_kernel(const PagedArgs a) {
       end = 1;
       const PagedSeq s(a, cut.b);
       if (s.nq == 0) return;
-      cut.lo = a.window >= 0 ? max(0, s.len - s.nq - a.window) & ~(kFewUnit - 1) : 0;
+      cut.lo = a.window >= 0 ? max(0, s.pos0 - a.window) & ~(kFewUnit - 1) : 0;
     } else if (rest >= 0) {
       if (rest == cut.total) ++h, rest = 0;
       cut.pass(a, rest);
@@ -175,7 +175,7 @@ void paged_few_kernel(const PagedArgs a) {
     n = min(cut.units - f, end - pos);
     const int b = uniform(cut.b);
     const PagedSeq s(a, b);
-    const int rows = s.nq * a.g, pos0 = s.len - s.nq;
+    const int rows = s.nq * a.g, pos0 = s.pos0;
     // not cut (also where nothing joins: keys or rows beyond the caller's bounds): all of it where it starts
     const bool whole = n == cut.units || !a.split || rows > a.part_rows;
     if (whole && f > 0) continue;
@@ -216,7 +216,7 @@ void paged_few_kernel(const PagedArgs a) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int j = j0 + 16 * u;
-          const bool has = page[u] >= 0 && page[u] < a.c.pages;
+          const bool has = page[u] >= 0 && page[u] < a.c.pages && j < s.len;
           const uint32_t bit = 1u << (2 * (t & 15) + u);
           held = has ? held | bit : held & ~bit;
           d.template issue<true>(slot + 16 * u * D, has ? page[u] : -1, j & ((1 << a.shift) - 1), t < nt ? s.len - j : 0);

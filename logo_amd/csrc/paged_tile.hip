@@ -209,7 +209,7 @@ struct TilePages {
         int v = -1;
         if (j < len && e < width) v = row[e];
         const bool held = v >= 0 && v < pages;
-        ok[u] = __ballot(held || j >= len);  // keys behind the last one are masked by position
+        ok[u] = __ballot(held);
         if (u == own) id = held ? v : -1;
       }
     }
@@ -269,7 +269,7 @@ void paged_tile_kernel(const PagedArgs a) {
   TileWork w;
   if (!w.find(a, rank, ROWS, true)) return;
   const PagedSeq s(a, w.b);
-  const int r0 = w.tile * ROWS, pos0 = s.len - s.nq;
+  const int r0 = w.tile * ROWS, pos0 = s.pos0;
   // token in the sequence of row r
   auto token = [&](int r) {
     const int t = a.g == 1 ? r : (int)((uint32_t)r / (uint32_t)a.g);
@@ -288,7 +288,7 @@ void paged_tile_kernel(const PagedArgs a) {
   // the keys that the workgroup's rows see, of its piece
   const int W = a.window;
   int kv_lo = WINDOW ? max(0, pos0 + uniform(token(r0)) - W) & ~63 : 0;
-  int kv_hi = pos0 + uniform(token(rl)) + 1;
+  int kv_hi = min(s.len, pos0 + uniform(token(rl)) + 1);
   if (w.npiece > 1) {
     kv_lo = w.piece * w.chunk;
     if (w.piece < w.npiece - 1) kv_hi = min(kv_hi, kv_lo + w.chunk);
@@ -551,7 +551,7 @@ __global__ __launch_bounds__(256) void paged_tile_join_kernel(const PagedArgs a)
   const int r = w.tile * ROWS + blockIdx.x % (ROWS / kJoinRows) * kJoinRows + threadIdx.x / LANES;
   const int col = threadIdx.x % LANES * V;
   if (r >= w.rows) return;
-  const int tok = a.sel ? a.idx[s.lo + r / a.g] : r / a.g, p = s.len - s.nq + tok;
+  const int tok = a.sel ? a.idx[s.lo + r / a.g] : r / a.g, p = min(s.len - 1, s.pos0 + tok);
   // pieces that hold keys which the row sees
   const int np = p < 0 ? 0 : min(p / w.chunk, w.npiece - 1) + 1;
   const int64_t size = (int64_t)ROWS * paged_part_row(D), step = w.total * size;

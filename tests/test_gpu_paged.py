@@ -338,6 +338,23 @@ def test_wrong_bounds_cost_time_only(gpu, bounds):
     ref.check("o", o, r, ref.attn_bound(r, mag, F16))
 
 
+@pytest.mark.parametrize("new,lens,cols", [([10, 3], [70, 50], 4), ([1, 1, 1], [40, 1100, 2000], 62), ([200, 5], [1400, 90], 75),
+                                           ([150, 700], [2100, 2500], 131), ([2, 40], [33, 77], 0)])
+@pytest.mark.parametrize("kw", [dict(), dict(window=20), dict(window=900)], ids=lambda k: str(k.get("window")))
+def test_lens_beyond_the_table(gpu, new, lens, cols, kw):
+    """Keys behind the block table have no page: tokens keep their positions and see what the table reaches."""
+    g = gen(40)
+    kp, vp, table, cu, ln = ref.paged_inputs(new, lens, 2, 64, 16, BF16, g)
+    q = torch.randn(sum(new), 4, 64, generator=g).to(BF16)
+    wide = table.clone()
+    wide[:, cols:] = -1
+    r, mag = ref.paged_attn(q, kp, vp, wide, cu, ln, **kw)
+    pools = [kp.to(gpu), vp.to(gpu)]
+    for bounds in ({}, dict(max_q=max(new), max_len=max(lens))):
+        o = paged_attn(q.to(gpu), *pools, table[:, :cols].to(gpu), cu.to(gpu), ln.to(gpu), **bounds, **kw)
+        ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
+
+
 def test_pages_beyond_32_bits(gpu):
     """Pages 3 GB apart: element and byte offsets past 2^32."""
     D, H, page, stride = 64, 2, 16, 3 << 29
