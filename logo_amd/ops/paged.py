@@ -44,8 +44,9 @@ def paged_append(k, v, k_pages, v_pages, block_table, cu_seqlens, lens, q=None, 
     Tokens behind the last sequence are not stored and have zero rows in the
     result, like tokens at negative positions; a token behind the block table or
     on an entry that names no page is not stored.  Two tokens of one call must not
-    share a slot (sequences may share pages that the call does not write)."""
-    _no_grad("paged_append", k, v, q)
+    share a slot (sequences may share pages that the call does not write), and no
+    two rows of the pages the same memory."""
+    _no_grad("paged_append", k, v, q, k_pages, v_pages)
     rot = (None, 0, 0, False, 1.0) if plan is None else (plan.turns, plan.head_dim, plan.rot_dim, plan.interleaved,
                                                          plan.amplitude)
     out = _torch_ops.timed("logo_paged_append", _torch_ops.ops().paged_append, k, v, k_pages, v_pages, block_table,
@@ -66,9 +67,9 @@ def paged_attn(q, k_pages, v_pages, block_table, cu_seqlens, lens, max_q: Option
     keys of one sequence from the host (defaults: N and the block table's reach);
     they choose the kernel, and larger device values cost time only.  ``scale``
     defaults to ``D ** -0.5``.  Returns ``[N, HQ, D]``; rows behind the last sequence
-    are zero, or left as they are in an ``out`` of the caller's (contiguous).  No
-    gradients."""
-    _no_grad("paged_attn", q)
+    are zero, or left as they are in an ``out`` of the caller's (contiguous; q itself,
+    or apart from all inputs).  No gradients."""
+    _no_grad("paged_attn", q, k_pages, v_pages, out)
     if window is not None and window < 0:
         raise ValueError(f"paged_attn: window must be None or >= 0, got {window}")
     args = (q, k_pages, v_pages, block_table, cu_seqlens, lens, selection, -1 if max_q is None else max(0, max_q),

@@ -371,6 +371,37 @@ int float_code(at::ScalarType t) {
 // Stride of dimension d, 0 where its size makes it meaningless.
 int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
+// Whether no two rows (last dimension) of x share memory: from the smallest stride up,
+// each dimension steps over what the ones before it span.
+bool rows_apart(const at::Tensor& x) {
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int64_t d = 0; d < x.dim() - 1; ++d)
+    if (x.size(d) > 1) dims.emplace_back(x.stride(d), x.size(d));
+  std::sort(dims.begin(), dims.end());
+  int64_t extent = x.size(-1);
+  for (const auto& [st, n] : dims) {
+    if (st < extent) return false;
+    extent += st * (n - 1);
+  }
+  return true;
+}
+
+// Whether the stretches of memory that x and y lie in overlap.
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return static_cast<const char*>(x.data_ptr()) < end(y) && static_cast<const char*>(y.data_ptr()) < end(x);
+}
+
+// What was written in place is another version to autograd.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // Shapes and types of a paged cache and a call's sequences.
@@ -390,7 +421,7 @@ void check_cache(const char* what, const at::Tensor& k_pages, const at::Tensor& 
   NEED(page >= 16 && page <= 65536 && (page & (page - 1)) == 0, what,
        ": page_size must be a power of two in [16, 65536], got ", page);
   for (const at::Tensor* t : {&k_pages, &v_pages})
-    NEED(t->stride(3) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0 &&
+    NEED(t->stride(3) == 1 && stride_of(*t, 0) % 8 == 0 && stride_of(*t, 1) % 8 == 0 && t->stride(2) % 8 == 0 &&
              t->stride(2) >= D && aligned16(*t),
          what, ": rows of the pages must be dense and 16-byte aligned");
 }
@@ -400,8 +431,8 @@ logo_paged_cache cache_arg(const at::Tensor& k_pages, const at::Tensor& v_pages,
   logo_paged_cache c{};
   c.k = k_pages.data_ptr();
   c.v = v_pages.data_ptr();
-  c.k_page = k_pages.stride(0), c.k_head = k_pages.stride(1), c.k_slot = k_pages.stride(2);
-  c.v_page = v_pages.stride(0), c.v_head = v_pages.stride(1), c.v_slot = v_pages.stride(2);
+  c.k_page = stride_of(k_pages, 0), c.k_head = stride_of(k_pages, 1), c.k_slot = k_pages.stride(2);
+  c.v_page = stride_of(v_pages, 0), c.v_head = stride_of(v_pages, 1), c.v_slot = v_pages.stride(2);
   c.pages = k_pages.size(0);
   c.heads = (int32_t)k_pages.size(1);
   c.page_size = (int32_t)k_pages.size(2);
@@ -414,7 +445,10 @@ logo_paged_cache cache_arg(const at::Tensor& k_pages, const at::Tensor& v_pages,
   return c;
 }
 
-at::Tensor dense_columns(const at::Tensor& t) { return t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t; }
+// The block table with dense rows, one behind the other.
+at::Tensor dense_table(const at::Tensor& t) {
+  return (t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1)) ? t.contiguous() : t;
+}
 
 // x [N, H, D] with rows that 16-byte accesses reach (a copy where they do not).
 at::Tensor rows16(const at::Tensor& x) {
@@ -441,11 +475,18 @@ at::Tensor paged_attn_impl(const at::Tensor& q_in, const at::Tensor& k_pages, co
   NEED(!out_in.has_value() || (out_in->sizes() == q_in.sizes() && out_in->scalar_type() == q_in.scalar_type() &&
                                out_in->is_contiguous() && aligned16(*out_in)),
        what, ": out must be contiguous, of q's shape and type");
+  if (out_in.has_value()) {
+    // q itself is fine: each row is read before its result is written, by the workgroups that need it
+    const bool same = out_in->data_ptr() == q_in.data_ptr() && q_in.is_contiguous();
+    NEED((same || !overlap(*out_in, q_in)) && !overlap(*out_in, k_pages) && !overlap(*out_in, v_pages), what,
+         ": out overlaps an input");
+  }
   on_gpu(what, {&k_pages, &v_pages, &table_in, &cu_in, &lens_in, &q_in, optional_ptr(selection), optional_ptr(out_in)});
   const c10::OptionalDeviceGuard guard(k_pages.device());
+  if (out_in.has_value()) written(*out_in);
   at::Tensor out = out_in.has_value() ? *out_in : at::empty({N, HQ, D}, q_in.options());
   if (N == 0 || HQ == 0) return out;
-  const at::Tensor q = rows16(q_in), table = dense_columns(table_in), cu = cu_in.contiguous(), lens = lens_in.contiguous();
+  const at::Tensor q = rows16(q_in), table = dense_table(table_in), cu = cu_in.contiguous(), lens = lens_in.contiguous();
   const at::Tensor sel = selection.has_value() ? selection->contiguous() : at::Tensor();
   const logo_paged_cache c = cache_arg(k_pages, v_pages, table, cu, lens);
   const int64_t reach = (int64_t)c.table_width * c.page_size;
@@ -496,13 +537,17 @@ at::Tensor paged_append(const at::Tensor& k_in, const at::Tensor& v_in, const at
                              q_in->scalar_type() == k_in.scalar_type()),
        what, ": q must be [N, HQ, D] of k's type");
   const uint64_t* tp = turns.has_value() ? check_plan(what, D, *turns, head_dim, rot) : nullptr;
+  NEED(rows_apart(k_pages) && rows_apart(v_pages) && (k_pages.numel() == 0 || k_pages.data_ptr() != v_pages.data_ptr()),
+       what, ": rows of the pages share memory");
   on_gpu(what, {&k_pages, &v_pages, &table_in, &cu_in, &lens_in, &k_in, &v_in, optional_ptr(q_in), optional_ptr(turns)});
   const c10::OptionalDeviceGuard guard(k_pages.device());
+  written(k_pages);
+  written(v_pages);
   const int64_t HQ = q_in.has_value() ? q_in->size(1) : 0;
   at::Tensor out = at::empty({q_in.has_value() ? N : 0, HQ, D}, k_in.options());
   if (N == 0 || k_in.size(1) == 0) return out;
   const at::Tensor k = rows16(k_in), v = rows16(v_in), q = HQ > 0 ? rows16(*q_in) : at::Tensor();
-  const at::Tensor table = dense_columns(table_in), cu = cu_in.contiguous(), lens = lens_in.contiguous();
+  const at::Tensor table = dense_table(table_in), cu = cu_in.contiguous(), lens = lens_in.contiguous();
   if (lens.size(0) == 0) return out.zero_();
   const logo_paged_cache c = cache_arg(k_pages, v_pages, table, cu, lens);
   ok(logo_paged_append(&c, cptr(k), stride_of(k, 0), stride_of(k, 1), cptr(v), stride_of(v, 0), stride_of(v, 1),
@@ -641,18 +686,12 @@ void rotary_(at::TensorList xs, const at::Tensor& positions, const at::Tensor& t
   std::vector<at::Tensor> rows;
   for (const at::Tensor& x : xs) {
     NEED(x.dim() <= 4 && (x.size(-1) <= 1 || x.stride(-1) == 1), "rotary_ needs [T, H, D] or [B, T, H, D] tensors with dense rows");
-    // from the smallest stride up, each dimension must step over what the ones before it span
-    std::vector<std::pair<int64_t, int64_t>> dims;
-    for (int64_t d = 0; d < x.dim() - 1; ++d)
-      if (x.size(d) > 1) dims.emplace_back(x.stride(d), x.size(d));
-    std::sort(dims.begin(), dims.end());
-    int64_t extent = x.size(-1);
-    for (const auto& [st, n] : dims) {
-      NEED(st >= extent, "rotary_: rows share memory");
-      extent += st * (n - 1);
-    }
+    bool apart = rows_apart(x);
+    for (const at::Tensor& y : rows) apart = apart && (x.numel() == 0 || x.data_ptr() != y.data_ptr());
+    NEED(apart, "rotary_: rows share memory");
     rows.push_back(x);
   }
+  for (const at::Tensor& x : xs) written(x);
   const c10::OptionalDeviceGuard guard(positions.device());
   launch_rotary(rows, rows, xs[0].sizes().slice(0, xs[0].dim() - 2), positions, turns, rot, interleaved, amplitude, false);
 }

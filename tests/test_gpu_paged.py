@@ -433,6 +433,44 @@ def test_append_captured_with_attention(gpu):
         assert torch.equal(a.nan_to_num(), b.nan_to_num())
 
 
+def test_views_of_tables_and_pages(gpu):
+    """One table for all sequences as an expanded view, a single page or head of any stride, results written over q."""
+    g = gen(41)
+    kp, vp, table, cu, ln = ref.paged_inputs([3, 2, 40], [90, 90, 90], 1, 64, 128, BF16, g)
+    table[1:] = table[0]
+    N = 45
+    q = torch.randn(N, 4, 64, generator=g).to(BF16)
+    r, mag = ref.paged_attn(q, kp, vp, table, cu, ln)
+    page = int(table[0, 0])
+    pools = []
+    for p in (kp, vp):
+        rows = torch.empty_strided((1, 1, 128, 64), (12345, 777, 64, 1), dtype=BF16, device=gpu)
+        pools.append(rows.copy_(p[page:page + 1]))
+    for big in (N, 8):  # both kernels
+        tb = torch.zeros(1, 1, dtype=torch.int32, device=gpu).expand(3, 1)
+        over = q.to(gpu)
+        o = paged_attn(over, *pools, tb, cu.to(gpu), ln.to(gpu), max_q=big)
+        ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
+        before = over._version
+        assert paged_attn(over, *pools, tb, cu.to(gpu), ln.to(gpu), max_q=big, out=over) is over
+        assert torch.equal(over, o) and over._version > before
+
+
+def test_append_is_seen_by_autograd(gpu):
+    """Pages saved for a backward pass and written since are an error there, as for any write in place."""
+    g = gen(42)
+    kp, vp, table, cu, ln = [t.to(gpu) for t in ref.paged_inputs([2], [20], 1, 64, 16, BF16, g)]
+    w = torch.ones(1, device=gpu, dtype=BF16, requires_grad=True)
+    y = (kp * w).sum()
+    k = torch.randn(2, 1, 64, generator=g).to(BF16).to(gpu)
+    paged_append(k, k, kp, vp, table, cu, ln)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        kp2, vp2 = kp.clone(), vp.clone()
+        paged_append(k, k, kp2, vp2, table, cu, ln)
+
+
 def test_operator_registrations(gpu):
     """torch.library's checks of the operators: schemas, fakes, autograd registration."""
     from logo_amd import _torch_ops

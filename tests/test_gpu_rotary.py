@@ -188,3 +188,17 @@ def test_captured_training_pass_and_streams(gpu):
         for a, b in zip(out, step()):
             assert torch.equal(a, b), k
     assert not torch.equal(eager[0], out[0])
+
+
+def test_in_place_writes(gpu):
+    """The same tensor twice is refused; a tensor saved for a backward pass and rotated since is an error there."""
+    plan = rotary_plan(64, device=gpu)
+    x = torch.randn(1, 5, 2, 64, device=gpu)
+    pos = torch.arange(5, device=gpu)
+    with pytest.raises(ValueError, match="share memory"):
+        rotary_([x, x], pos, plan)
+    w = torch.ones(1, device=gpu, requires_grad=True)
+    y = (x * w).sum()
+    rotary_([x], pos, plan)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

@@ -119,6 +119,26 @@ def test_attn_refusals(kw, msg):
         paged_attn(**_args())
 
 
+def test_shared_memory_refusals():
+    """Memory that a call would write and read, or write twice."""
+    a = _args()
+    both = torch.zeros(5, 8, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="out overlaps"):
+        paged_attn(**{**a, "q": both[:, 4:].transpose(0, 1).contiguous().transpose(0, 1), "out": a["k_pages"].view(-1)[:1280].view(5, 4, 64)})
+    line = torch.zeros(2000, dtype=BF16)
+    with pytest.raises(ValueError, match="out overlaps"):
+        paged_attn(**{**a, "q": line[:1280].view(5, 4, 64), "out": line[64:1344].view(5, 4, 64)})
+    for kw in (dict(v_pages=a["k_pages"]), dict(k_pages=a["k_pages"][:, :1].expand(6, 2, 16, 64)),
+               dict(v_pages=a["k_pages"][:1].clone().expand(6, 2, 16, 64))):
+        with pytest.raises(ValueError, match="share memory"):
+            b = {**a, **kw}
+            q = b.pop("q")
+            paged_append(q[:, :2], q[:, :2], **b)
+    for name in ("k_pages", "v_pages"):
+        with pytest.raises(ValueError, match="no gradients"):
+            paged_attn(**{**a, name: a[name].clone().requires_grad_()})
+
+
 def test_append_refusals():
     a = _args()
     q = a.pop("q")
