@@ -537,19 +537,21 @@ void paged_tile_kernel(const PagedArgs a) {
   }
 }
 
-// Joins the pieces of eight rows of a row tile a workgroup.
-constexpr int kJoinRows = 8;
+// Joins the pieces of some rows of a row tile a workgroup, eight lanes a row.  Each
+// workgroup first finds its tile (some 3 us), so it takes 32 rows and not fewer: at 8 the
+// launch took 18.9 us for a batch of 12 single tokens and four chunks of 500 behind up to
+// 8192 keys (16 heads, D = 64; 24 MB of partial results), at 32 9.2 us.
+constexpr int kJoinRows = 32;
 template <typename EL, int D, int NW>
 __global__ __launch_bounds__(256) void paged_tile_join_kernel(const PagedArgs a) {
-  constexpr int ROWS = 32 * NW, LANES = 256 / kJoinRows, V = D / LANES;  // 4 or 2 columns a lane
-  typedef float fv __attribute__((ext_vector_type(V)));
-  typedef EL ev __attribute__((ext_vector_type(V)));
+  constexpr int ROWS = 32 * NW, LANES = 256 / kJoinRows, CT = D / (4 * LANES);  // four columns of CT a lane
+  using E4 = typename Elem<EL>::x4;
   const int h = blockIdx.y;
   TileWork w;
   if (!w.find(a, blockIdx.x / (ROWS / kJoinRows), ROWS, false) || w.npiece == 1) return;
   const PagedSeq s(a, w.b);
   const int r = w.tile * ROWS + blockIdx.x % (ROWS / kJoinRows) * kJoinRows + threadIdx.x / LANES;
-  const int col = threadIdx.x % LANES * V;
+  const int col = threadIdx.x % LANES * 4;
   if (r >= w.rows) return;
   const int tok = a.sel ? a.idx[s.lo + r / a.g] : r / a.g, p = min(s.len - 1, s.pos0 + tok);
   // pieces that hold keys which the row sees
@@ -560,19 +562,30 @@ __global__ __launch_bounds__(256) void paged_tile_join_kernel(const PagedArgs a)
   float m = -INFINITY;
   for (int k = 0; k < np; ++k) m = fmaxf(m, pp[k * step + D]);
   const float base = m == -INFINITY ? 0.f : m;
-  fv o = fv{};
+  f32x4 o[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) o[c] = f32x4{};
   float sum = 0.f;
+#pragma unroll 2
   for (int k = 0; k < np; ++k) {
-    const float f = fast_exp2(pp[k * step + D] - base);
-    sum = fmaf(f, pp[k * step + D + 1], sum);
-    const fv x = *reinterpret_cast<const fv*>(pp + k * step + col);
+    const float* const pk = pp + k * step;
+    const float f = fast_exp2(pk[D] - base);
+    sum = fmaf(f, pk[D + 1], sum);
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = fmaf(f, x[e], o[e]);
+    for (int c = 0; c < CT; ++c) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(pk + 4 * LANES * c + col);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[c][e] = fmaf(f, x[e], o[c][e]);
+    }
   }
-  ev v;
+  EL* const orow = reinterpret_cast<EL*>(a.out) + ((s.lo + tok) * a.hq + h * a.g + r % a.g) * D + col;
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = (EL)(sum != 0.f ? o[e] / sum : 0.f);
-  *reinterpret_cast<ev*>(reinterpret_cast<EL*>(a.out) + ((s.lo + tok) * a.hq + h * a.g + r % a.g) * D + col) = v;
+  for (int c = 0; c < CT; ++c) {
+    E4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (EL)(sum != 0.f ? o[c][e] / sum : 0.f);
+    *reinterpret_cast<E4*>(orow + 4 * LANES * c) = v;
+  }
 }
 
 template <typename EL, int D, int NW>
