@@ -593,8 +593,11 @@ size_t logo_paged_attn_workspace_bytes(int nseq, int h, int hq, int64_t n_tokens
  * be null): a token whose entry is zero reads no key and gets zero rows (LoGo's
  * gate, logo/layers/logo.py:186-209, :228-249).  Rows that see no key are zero.
  * Rows behind the last sequence are zero with zero_rest, else left as they are.
- * max_q, max_len: bounds on the new tokens and on the keys of a sequence, which
- * size the launch; larger ones on the device stay right but slow.
+ * Keys behind the table or on an entry that names no page are not seen.  out may be
+ * q where q is dense, else it lies apart from all inputs.  max_q, max_len: bounds on
+ * the new tokens and on the keys of a sequence, which choose the kernel and how finely
+ * keys are cut; larger ones on the device stay right but slow.  nseq at most 65534, and
+ * nseq x heads x (table_width x page_size / 64 + 1) below 2^31.
  */
 int logo_paged_attn(const logo_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head, void* out,
                     const uint8_t* selection, int hq, int64_t n_tokens, int d, int max_q, int max_len, float scale,

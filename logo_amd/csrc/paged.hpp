@@ -73,6 +73,10 @@ struct PagedSeq {
     len = min(all, a.c.table_width << a.shift);
     pos0 = all - nq;
   }
+  // The first key that the token at position pos0 + t sees, in whole units of 64, at most len.
+  __device__ __forceinline__ int first_key(int t, int window) const {
+    return (int)max((int64_t)0, min((int64_t)pos0 + t - window, (int64_t)len)) & ~63;
+  }
 };
 
 // Copies of one kv head's rows into a kSwz tile, ROWS (8 or 16) at a time: rows row0

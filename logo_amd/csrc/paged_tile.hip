@@ -16,7 +16,7 @@ template <int D>
 constexpr size_t tile_smem() { return (size_t)4 * 64 * D * sizeof(bf16); }  // K and V, two of each
 
 // Selected tokens of each sequence, in order: one workgroup a sequence, 16 tokens a
-// thread and step.
+// thread and step (5 us for 8192 tokens, a launch's own time).
 constexpr int kSelThreads = 1024;
 __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedArgs a) {
   const int b = blockIdx.x, tid = threadIdx.x, l = tid & 63, wave = tid >> 6;
@@ -226,7 +226,18 @@ struct TilePages {
 // exponentials of P(t) spread over the first three quarters of the slots, the mask and
 // row maximum of S(t + 1) over the second half, and operand reads four slots ahead.
 // K is copied one tile further ahead than V.  A row's reference maximum moves only when
-// its maximum grew by more than 2^8 (or on its first key), so O is rarely rescaled.
+// its maximum grew by more than 2^8 (or on its first key), so O is rarely rescaled.  The
+// weights are rounded to the element type for the product with V (half a step of sum
+// w |v|, as much as the result's own rounding), their sum is not.
+//
+// Bound by the MFMAs and the vector work beside them: 16384 tokens behind 16384 (16 heads
+// over 4, D = 128) take 3.1 ms, 1060 TFLOP/s, with the MFMAs 51% busy, the vector units 49%
+// and 32% of wave time waiting; the dense causal kernel of this library reaches 1100 at
+// 16384 tokens of 16 heads.  At D = 64 a score has half the MFMA work for the same vector
+// work: 590 TFLOP/s (four chunks of 512 behind 7680).  Windows and short pieces are bound
+// by a workgroup's start (3 to 6 us: its place, its pages, the first tiles) and the
+// latency of a step: 4 x 2048 tokens with a window of 128 (16 heads) 49 us.  The same loop
+// without the pipeline: 7.4 ms for the first, 97 us for the last.
 template <typename EL, int D, bool WINDOW, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_tile_kernel(const PagedArgs a) {
@@ -287,7 +298,7 @@ void paged_tile_kernel(const PagedArgs a) {
   pin(pmax);
   // the keys that the workgroup's rows see, of its piece
   const int W = a.window;
-  int kv_lo = WINDOW ? max(0, pos0 + uniform(token(r0)) - W) & ~63 : 0;
+  int kv_lo = WINDOW ? s.first_key(uniform(token(r0)), W) : 0;
   int kv_hi = min(s.len, pos0 + uniform(token(rl)) + 1);
   if (w.npiece > 1) {
     kv_lo = w.piece * w.chunk;
@@ -320,7 +331,7 @@ void paged_tile_kernel(const PagedArgs a) {
     d.issue(tile + RPW * wave * D, page, j & ((1 << a.shift) - 1), s.len - j);
   };
   const int tw_hi = active ? min(nt, ((pmax - kv_lo) >> 6) + 1) : 0;  // the wave's tiles
-  const int tw_lo = WINDOW && active ? max(0, pmin - W - kv_lo) >> 6 : 0;
+  const int tw_lo = WINDOW && active ? max(0, max(pmin, 0) - W - kv_lo) >> 6 : 0;
   int page_v = -1;              // page of the wave's rows of tile t + 1
   uint32_t bad1 = 0, bad2 = 0;  // groups without a page of tiles t + 1 and t + 2
   bool edge = false;            // tile t crosses the edge of some row's keys
@@ -618,7 +629,8 @@ static int tile_dispatch(const PagedArgs& a, int h, int nw, hipStream_t st) {
 }
 
 // Eight waves (256 rows share a tile's copies) where at least two rounds of such
-// workgroups are sure, one on a CU; four elsewhere, two on a CU.
+// workgroups are sure, one on a CU; four elsewhere, two on a CU.  16384 tokens behind
+// 16384 (16 heads over 4, D = 128): 3140 us with eight, 3530 with four.
 void tile_plan(int nseq, int h, int g, int64_t n, int64_t span, int cus, bool sel, bool& split, int& target, int& cap,
                int& nw) {
   const int64_t rows = n * g;

@@ -19,7 +19,15 @@
 // tokens of one tensor; cos and sin of its tokens are worked out once into LDS
 // and serve all heads.  A thread keeps its place in the row and walks the rows, two
 // in flight at a time; the first two are on their way before the tokens' positions
-// are known.
+// are known.  Loads and stores are streaming (nothing is read again).
+//
+// Measured: 4 x 8192 tokens of 16 + 4 heads of 128 in bf16, 336 MB a pass in 60 us (5.6
+// TB/s; a large copy with streaming loads and stores 5.9), the training step's two
+// passes 121 us; 32K keys and values of 4 heads and 16 query heads of 128 in fp16
+// appended and rotated, 306 MB in 57 us; a decode step of 8 or 32 sequences 5 to 6 us, a
+// launch's own time.  Workgroups of 1024 items: of 256, which pay for their tokens'
+// angles, the training step takes 128 us and the append 90, of 4096 128 and 62.  Two
+// items in flight: one takes 126 and 57 us, four 119 and 69.
 #include <math.h>
 
 #include <algorithm>

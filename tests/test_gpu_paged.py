@@ -355,6 +355,25 @@ def test_lens_beyond_the_table(gpu, new, lens, cols, kw):
         ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
 
 
+@pytest.mark.parametrize("length", [1 << 30, (1 << 31) - 1])
+@pytest.mark.parametrize("window", [None, 40, 1 << 30, 1 << 40])
+@pytest.mark.parametrize("n,max_q", [(3, 3), (50, 50)])
+def test_positions_up_to_32_bits(gpu, n, max_q, window, length):
+    """Positions far behind the table: every key of the table is seen, or, with a window that ends behind it, none."""
+    g = gen(43)
+    kp, vp, table, cu, ln = ref.paged_inputs([n], [100], 2, 64, 16, BF16, g)
+    table = table[:, :6]  # 96 keys
+    q = torch.randn(n, 4, 64, generator=g).to(BF16)
+    all_keys = window is None or window > length
+    r, mag = ref.paged_attn(q, kp, vp, torch.nn.functional.pad(table, (0, 99), value=-1), cu, torch.tensor([1000]))
+    part = window == 1 << 30 and length == 1 << 30  # the first keys: p - 2^30 < 0 for all tokens
+    if not (all_keys or part):
+        r, mag = torch.zeros_like(r), torch.zeros_like(mag)
+    ln = torch.tensor([length], dtype=torch.int32, device=gpu)
+    o = paged_attn(q.to(gpu), kp.to(gpu), vp.to(gpu), table.to(gpu), cu.to(gpu), ln, max_q=max_q, window=window)
+    ref.check("o", o, r, ref.attn_bound(r, mag, BF16))
+
+
 def test_pages_beyond_32_bits(gpu):
     """Pages 3 GB apart: element and byte offsets past 2^32."""
     D, H, page, stride = 64, 2, 16, 3 << 29
