@@ -53,13 +53,14 @@ namespace logo {
 // Measured (D = 128): 32 sequences of up to 16384 keys, 16 heads in bf16, half of them
 // selected, 2.02 GB in 314 us (6.4 TB/s; a plain streaming read reaches 7.1); 3 x up to
 // 100003 keys, 32 heads over 4 in fp16, 462 MB in 80 us (5.7 TB/s) and the join 5.5; 700 keys
-// of 4 heads 18 us and the join 4, all of it latency.  Pieces of a fixed number of keys,
+// of 4 heads 15.6 us with the join, all of it latency.  Pieces of a fixed number of keys,
 // each with two tiles in flight, took 435 and 120 us.
 constexpr int kFewWaves = 2;
 constexpr int kFewUnit = 64;      // keys (as PagedSeq::first_key)
-constexpr int kFewMinShare = 4;   // units: the shortest stretch, unless a sequence ends
-// Keys up to which no sequence is cut.  One workgroup takes 8.1 us for 64 keys, 11.8 for
-// 256, 27.5 for 1024; cut in four, 1024 take 12.9 us and the launch that joins them 4.1.
+// Keys up to which no sequence is cut.  A call takes 14.9 us uncut and 16.4 cut with its
+// join for one sequence of 300 keys (4 heads), 18.3 and 15.4 for one of 512, 18.4 and 22.1
+// for 16 of 512 (16 heads).  Beyond it a stretch may be as short as a unit: of four at least,
+// 700 keys took 22.7 us and not 15.6, one sequence of 8000 22.4 and not 18.
 constexpr int kFewWhole = 512;
 
 template <int D>
@@ -115,7 +116,7 @@ struct FewCut {
       base += __builtin_amdgcn_readlane(pre, 63);
     }
     total = base;
-    share = max(kFewMinShare, (base * a.c.heads + a.target - 1) / a.target);
+    share = max(1, (base * a.c.heads + a.target - 1) / a.target);
   }
 };
 
